@@ -35,6 +35,7 @@ extern "C" {
 
 /* ---- device status bits (uwc_device_status) */
 #define UWC_DEV_TIMEOUT 1u /* a kernel's bounded wait ran out and the kernel unwound */
+#define UWC_DEV_RANGE 2u   /* a paged call's device-side metadata was out of range; what was out of it was skipped */
 
 /* ---- constants shared with the reference (ops.py:26-29, kernels.cu:475-480) */
 #define UWC_FLAG_HASH 1
@@ -431,6 +432,61 @@ int uwc_stage_out_leaves(const float* rows, long long nrows, int D, int T, uint3
  * (runtime/detgpu/sha.py:138-163), agent.proto.stage_output_root per stage. */
 int uwc_stage_roots(const float* rows, int B, int T, int D, uint32_t* scratch, uint64_t scratch_words,
                     uint32_t* roots, void* stream);
+
+/* ---- the paged 8-bit KV cache ------------------------------------------------------------------
+ * New (the reference keeps one contiguous cache per batch, runtime/detrt/qwen3.py:216-221). One
+ * layer's cache is a pool of pages: k, v (pages, Hkv, page_size, 128) int8, 16-byte aligned, and sk,
+ * sv (pages, Hkv) float32, the scale of each (page, KV head); page_size 16, 32, 64 or 128. A cached
+ * value is its integer times its page's scale.
+ * A batch is ragged and described on the device, so one CUDA graph serves every step: rows cu[s] ..
+ * cu[s + 1] - 1 of the row tensors are sequence s's new tokens (none where the two are equal) at
+ * positions start[s] and on, and table (seqs x width int32, row-contiguous) lists its pages: position
+ * p lies in page table[s][p / page_size]. start[s] < 0 marks an idle slot: nothing is written to the
+ * cache for it, and its rows come out zero. Entries of the table past a sequence's last position are
+ * not read. Host-side bounds: rows = the row tensors' length, max_new >= every sequence's new tokens,
+ * max_len >= every start[s] + new tokens (attention; sizes the split, exceeding it is safe but slow).
+ * Metadata out of its range (a page outside the pool, a position past the table or the rotation
+ * table, rows past `rows`, more than max_new new tokens) is skipped and raises UWC_DEV_RANGE in
+ * uwc_device_status. Rows that no sequence covers are not written. A page may be shared by several
+ * tables (a common prefix) as long as no call appends to it from more than one.
+ * dtype: UWC_T_BF16 or UWC_T_F16, of every row tensor of the call. Row tensors may be strided: element
+ * (n, h, d) at n * tok + h * head + d; strides are multiples of 8 elements, base pointers 16-byte aligned. */
+#define UWC_T_BF16 0
+#define UWC_T_F16 1
+#define UWC_T_F32 2 /* uwc_paged_gather's output only */
+/* Rotate and append: the new tokens' keys k (rows, Hkv, 128), rotated with rows `position` of cos / sin
+ * ((max_pos, 128) float32, the layout of uwc_qkv_post_at's tables), and values v, quantized into their
+ * pages; with q != NULL the queries (rows, H, 128) rotated into q_out (contiguous). q_norm / k_norm
+ * (128 float32 or NULL): det_rmsnorm of each head with eps before the rotation (Qwen3).
+ * A page's scale is max(the scale of the tokens it already holds, max|new values| / 127); the tokens it
+ * already holds are brought to a grown scale (rint(q * old / new)). Positions before start[s] in the
+ * page of start[s] count as held; a page entered at its first position starts anew. Each step is one
+ * IEEE float32 operation. Infinities are stored as +-127 and NaN as 0; neither counts toward the scale. */
+int uwc_paged_append(int8_t* kc, float* sk, int8_t* vc, float* sv, int pages, int page_size, int Hkv,
+                     const int* table, const int* start, const int* cu, int seqs, int width, int rows, int max_new,
+                     int dtype, const void* k, long long k_tok, long long k_head, const void* v, long long v_tok,
+                     long long v_head, const void* q, long long q_tok, long long q_head, void* q_out, int H,
+                     const float* cos, const float* sin, int max_pos, const float* q_norm, const float* k_norm,
+                     double eps, void* stream);
+/* The cached tokens at positions first[s] .. as values (integer times scale, in dtype) into k, v
+ * (rows, Hkv, 128), rows cu[s] .. cu[s + 1] - 1 for sequence s, at most max_rows each. */
+int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t* vc, const float* sv, int pages, int page_size,
+                     int Hkv, const int* table, const int* first, const int* cu, int seqs, int width, int rows,
+                     int max_rows, int dtype, void* k, void* v, void* stream);
+/* Attention of the new tokens over their sequence's pages, which already hold them: the query at
+ * position p sees key j when j <= p and (window < 0, or j > p - window, or j < sinks). q (rows, H, 128),
+ * H a multiple of Hkv (head h reads KV head h / (H / Hkv)); out (rows, H, 128) contiguous, in dtype.
+ * softmax(scale q . k) in float32; a row that sees no key is zero. No atomics touch a result: the same
+ * call gives the same bits. workspace: uwc_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ * zero before its first use; every call leaves its counters zero again. Calls that overlap on the GPU
+ * must not share one. */
+uint64_t uwc_paged_attention_workspace_bytes(int seqs, int max_new, int max_len, int H, int Hkv, int window,
+                                             int sinks);
+int uwc_paged_attention(const int8_t* kc, const float* sk, const int8_t* vc, const float* sv, int pages, int page_size,
+                        int Hkv, const int* table, const int* start, const int* cu, int seqs, int width, int rows,
+                        int max_new, int max_len, int dtype, const void* q, long long q_tok, long long q_head,
+                        void* out, int H, float scale, int window, int sinks, void* workspace,
+                        uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

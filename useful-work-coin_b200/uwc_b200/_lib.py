@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "libuwcb200.so")
 
 OK, ERR_ARG, ERR_SHAPE, ERR_ALIGN, ERR_CUDA, ERR_DEVICE, ERR_SCRATCH = range(7)
 DEV_TIMEOUT = 1
+DEV_RANGE = 2
 HOOK_WAIT_NS, HOOK_WITHHOLD, HOOK_STREAM_PDL, HOOK_TP_TWO_PHASE = 1, 2, 3, 4
 
 # (name, restype, argtypes) for every function declared in include/uwc_b200.h
@@ -84,6 +85,12 @@ SIGNATURES = {
     "uwc_stage_scratch_words": (_U64, [_I64, _I32]),
     "uwc_stage_out_leaves": (_I32, [_P, _I64, _I32, _I32, _P, _U64, _P, _P]),
     "uwc_stage_roots": (_I32, [_P, _I32, _I32, _I32, _P, _U64, _P, _P]),
+    "uwc_paged_append": (_I32, [_P] * 4 + [_I32] * 3 + [_P] * 3 + [_I32] * 5 + [_P, _I64, _I64] * 3 + [_P, _I32, _P, _P,
+                                _I32, _P, _P, _F64, _P]),
+    "uwc_paged_gather": (_I32, [_P] * 4 + [_I32] * 3 + [_P] * 3 + [_I32] * 5 + [_P] * 3),
+    "uwc_paged_attention_workspace_bytes": (_U64, [_I32] * 7),
+    "uwc_paged_attention": (_I32, [_P] * 4 + [_I32] * 3 + [_P] * 3 + [_I32] * 6 + [_P, _I64, _I64, _P, _I32, _F32, _I32,
+                                   _I32, _P, _U64, _P]),
 }
 
 _LIB = None
@@ -125,7 +132,7 @@ def launch_count() -> int:
 
 
 def device_status(clear: bool = True) -> int:
-    """Sticky device-side error bits (DEV_TIMEOUT); synchronizes the current device."""
+    """Sticky device-side error bits (DEV_TIMEOUT, DEV_RANGE); synchronizes the current device."""
     v = ctypes.c_uint32(0)
     check(lib().uwc_device_status(ctypes.byref(v), 1 if clear else 0), "uwc_device_status")
     return int(v.value)
