@@ -59,7 +59,92 @@ __device__ __forceinline__ int page_at(const Seqs& b, const Cache& c, int s, int
   return id >= 0 && id < c.pages ? id : -1;
 }
 
+// ---- attention
+struct AttnArgs {
+  Cache c;
+  Seqs b;
+  const void* q;           // element (n, h, d) at n * q_tok + h * q_head + d
+  long long q_tok, q_head;
+  void* out;               // (rows, H, 128)
+  int H, window, sinks;    // window < 0: none
+  float scale;
+  uint32_t* status;
+};
+
+// The keys that tokens t0 .. t1 of a sequence see, as tiles of TILE keys: tiles 0 .. tA - 1 hold the
+// sinks, then tB0 .. on the windows. There is at least one tile, seen or not: it writes the zeros.
+template <int TILE>
+struct Keys {
+  int p0, p1;              // positions of the first and the last row
+  int lo, hi, sink_end;    // windows: keys lo .. hi - 1; sinks: keys below sink_end
+  int tA, tB0, total;
+  __device__ __forceinline__ Keys(const AttnArgs& a, const Span& sp, int t0, int t1) {
+    p0 = sp.idle ? -1 : sp.start + t0;
+    p1 = sp.idle ? -1 : sp.start + t1;
+    hi = a.window == 0 ? 0 : p1 + 1;
+    lo = a.window < 0 ? 0 : max(0, p0 - a.window + 1);
+    sink_end = a.window < 0 ? 0 : min(a.sinks, p1 + 1);
+    tA = (sink_end + TILE - 1) / TILE;
+    tB0 = max(tA, lo / TILE);
+    total = max(1, tA + max(0, (hi + TILE - 1) / TILE - tB0));
+  }
+  // the first key of tile i
+  __device__ __forceinline__ int key(int i) const { return (i < tA ? i : tB0 + (i - tA)) * TILE; }
+  // whether some row sees one of the n keys from j on
+  __device__ __forceinline__ bool seen(int j, int n) const { return j < sink_end || (j < hi && j + n > lo); }
+  // whether every row sees all of them
+  __device__ __forceinline__ bool full(const AttnArgs& a, int j, int n) const {
+    return j + n - 1 <= p0 && (a.window < 0 || j > p1 - a.window || j + n <= a.sinks);
+  }
+};
+__device__ __forceinline__ bool sees(const AttnArgs& a, int pos, int j) {
+  return j <= pos && (a.window < 0 || j > pos - a.window || j < a.sinks);
+}
+
+// Two 16-bit values as float32, and back.
+__device__ __forceinline__ float2 two_f(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 two_f(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two of four int8 values as an fp16 pair, exactly: with the values biased by 128 (the caller's
+// xor 0x80), 0x6400 | byte is the fp16 number 1024 + byte. sel 0x4140: bytes 0, 1; 0x4342: bytes 2, 3.
+__device__ __forceinline__ uint32_t i8_half2(uint32_t biased, uint32_t sel) {
+  const uint32_t h = __byte_perm(biased, 0x64646464u, sel), k = 0x64806480u;   // 1152, twice
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The exponent e that brings a row whose largest magnitude is mx to [2^14, 2^15): q 2^e is its fp16 form.
+__device__ __forceinline__ int row_exponent(float mx) {
+  const int x = (__float_as_int(mx) >> 23) & 255;
+  return mx == 0.f || x == 255 ? 0 : min(max(14 + 127 - x, -100), 100);
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+constexpr float kNoMax = -1e30f;             // a running maximum before any key
+constexpr float kLog2OfE = 1.4426950408889634f;
+
 }  // namespace paged
+
+// The form of uwc_paged_attention for more rows than the few-row form takes (paged_tile.cu).
+uint64_t uwc_paged_tile_workspace(int seqs, int max_new, int max_len, int H, int Hkv, int window, int sinks);
+int uwc_paged_tile_launch(const paged::AttnArgs* a, int dtype, int max_len, void* workspace, cudaStream_t stream);
+
+// Dynamic shared memory beyond 48 KiB, asked for once per kernel and device (paged_attn.cu).
+int uwc_paged_allow_smem(const void* kernel, int bytes);
 
 // The checks that every paged call shares (paged.cu).
 int uwc_paged_check(const paged::Cache* cache, const paged::Seqs* seqs);
