@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(const AppendArgs a) {
   const Span sp = span_of(a.b, a.c.ps, s);
   if (sp.bad && j == 0 && tid == 0) set_status(a.status, UWC_DEV_RANGE);
   if (sp.idle || sp.n <= 0) return;
-  const int ps = a.c.ps, slot = sp.start / ps + j, base = slot * ps;
+  const int ps = a.c.ps, slot = (sp.start >> a.c.lg) + j, base = slot * ps;
   const int p0 = max(sp.start, base), p1 = min(sp.start + sp.n, base + ps);   // positions written here
   if (p0 >= p1) return;
   const int page = page_at(a.b, a.c, s, slot);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_gather(const GatherArgs a) {
   const int t = (int)(u / a.c.Hkv), h = (int)(u % a.c.Hkv), c = threadIdx.x & 7;
   if (t >= sp.n) return;
   const int pos = sp.start + t, ps = a.c.ps;
-  const int page = sp.idle ? -1 : page_at(a.b, a.c, s, pos / ps);
+  const int page = sp.idle ? -1 : page_at(a.b, a.c, s, pos >> a.c.lg);
   if (page < 0 && !sp.idle) set_status(a.status, UWC_DEV_RANGE);
   const size_t out = ((size_t)(sp.row0 + t) * a.c.Hkv + h) * kHd + 16 * c;
 #pragma unroll
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_gather(const GatherArgs a) {
     float sc = 0.f;
     if (page >= 0) {
       const size_t ph = (size_t)page * a.c.Hkv + h;
-      w = *reinterpret_cast<const uint4*>((i ? a.c.v : a.c.k) + (ph * ps + pos % ps) * kHd + 16 * c);
+      w = *reinterpret_cast<const uint4*>((i ? a.c.v : a.c.k) + (ph * ps + (pos & (ps - 1))) * kHd + 16 * c);
       sc = (i ? a.c.sv : a.c.sk)[ph];
     }
     const uint32_t x[4] = {w.x, w.y, w.z, w.w};
@@ -321,14 +321,16 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 }  // namespace
 
 // The checks that every paged call shares: UWC_OK, or why not.
-int uwc_paged_check(const Cache* cache, const Seqs* seqs) {
-  const Cache& c = *cache;
+int uwc_paged_check(Cache* cache, const Seqs* seqs) {
+  Cache& c = *cache;
   const Seqs& b = *seqs;
   if (!c.k || !c.sk || !c.v || !c.sv || !b.table || !b.start || !b.cu) return UWC_ERR_ARG;
   if (c.pages < 1 || c.Hkv < 1 || (c.ps != 16 && c.ps != 32 && c.ps != 64 && c.ps != 128)) return UWC_ERR_SHAPE;
   if (b.seqs < 0 || b.seqs > 65535 || b.width < 1 || b.rows < 0 || b.max_new < 0) return UWC_ERR_SHAPE;
   if ((long long)b.width * c.ps > (1ll << 30) || b.rows > (1 << 30)) return UWC_ERR_SHAPE;
+  if ((long long)c.pages * c.Hkv * c.ps > 0x7fffffffll) return UWC_ERR_SHAPE;   // 256 GB of keys
   if (!aligned16(c.k) || !aligned16(c.v)) return UWC_ERR_ALIGN;
+  c.lg = c.ps == 16 ? 4 : c.ps == 32 ? 5 : c.ps == 64 ? 6 : 7;
   return UWC_OK;
 }
 
@@ -356,7 +358,7 @@ extern "C" int uwc_paged_append(int8_t* kc, float* sk, int8_t* vc, float* sv, in
                                 long long q_head, void* q_out, int H, const float* cos, const float* sin, int max_pos,
                                 const float* q_norm, const float* k_norm, double eps, void* stream) {
   AppendArgs a = {};
-  a.c = Cache{kc, sk, vc, sv, pages, page_size, Hkv};
+  a.c = Cache{kc, sk, vc, sv, pages, page_size, Hkv, 0};
   a.b = Seqs{table, start, cu, seqs, width, rows, max_new};
   const int rc = uwc_paged_check(&a.c, &a.b);
   if (rc != UWC_OK) return rc;
@@ -393,7 +395,7 @@ extern "C" int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t*
                                 int width, int rows, int max_rows, int dtype, void* k, void* v, void* stream) {
   GatherArgs a = {};
   a.c = Cache{const_cast<int8_t*>(kc), const_cast<float*>(sk), const_cast<int8_t*>(vc), const_cast<float*>(sv), pages,
-              page_size, Hkv};
+              page_size, Hkv, 0};
   a.b = Seqs{table, first, cu, seqs, width, rows, max_rows};
   const int rc = uwc_paged_check(&a.c, &a.b);
   if (rc != UWC_OK) return rc;

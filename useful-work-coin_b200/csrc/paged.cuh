@@ -22,6 +22,7 @@ struct Cache {
   int8_t* v;
   float* sv;
   int pages, ps, Hkv;
+  int lg;                  // log2 of ps
 };
 
 struct Seqs {
@@ -134,6 +135,31 @@ __device__ __forceinline__ int row_exponent(float mx) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
+// A wait of a whole warp in few instructions (a kernel of many roles lives on its instruction cache): up to
+// 2^23 polls, which take 0.1 us each while the barrier is not ready, so about a second. The same answer in
+// all lanes: false when it ran out.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t left = 1u << 23;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "POLL_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE_%=;\n\t"
+      "sub.u32 %0, %0, 1;\n\t"
+      "setp.ne.u32 p, %0, 0;\n\t"
+      "@p bra POLL_%=;\n\t"
+      "DONE_%=:\n\t}"
+      : "+r"(left)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xffffffffu, left != 0);
+}
+// One arrival for a warp, after all that its lanes did before.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 constexpr float kNoMax = -1e30f;             // a running maximum before any key
 constexpr float kLog2OfE = 1.4426950408889634f;
 
@@ -146,5 +172,5 @@ int uwc_paged_tile_launch(const paged::AttnArgs* a, int dtype, int max_len, void
 // Dynamic shared memory beyond 48 KiB, asked for once per kernel and device (paged_attn.cu).
 int uwc_paged_allow_smem(const void* kernel, int bytes);
 
-// The checks that every paged call shares (paged.cu).
-int uwc_paged_check(const paged::Cache* cache, const paged::Seqs* seqs);
+// The checks that every paged call shares; sets cache->lg (paged.cu).
+int uwc_paged_check(paged::Cache* cache, const paged::Seqs* seqs);

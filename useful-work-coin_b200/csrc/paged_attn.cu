@@ -77,6 +77,7 @@ __device__ __forceinline__ Part find_part(const AttnArgs& a) {
   const int lane = threadIdx.x & 31, S = a.b.seqs;
   long long sum = 0;
   int most = 0;
+#pragma unroll 1
   for (int s = lane; s < S; s += 32) {
     const int t = unit_of(a, s).total;
     sum += t;
@@ -91,6 +92,7 @@ __device__ __forceinline__ Part find_part(const AttnArgs& a) {
   p.count = min(p.per, p.total - p.first);
   if (p.count <= 0) return p;
   long long before = 0;
+#pragma unroll 1
   for (int s0 = 0; s0 < S; s0 += 32) {
     const long long t = s0 + lane < S ? (long long)unit_of(a, s0 + lane).total * a.c.Hkv : 0;
     long long inc = t;
@@ -159,6 +161,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
     tma_prefetch_desc(&mapV);
   }
   if (blockIdx.x == 0 && warp == kWarps)
+#pragma unroll 1
     for (int s = lane; s < a.b.seqs; s += 32)
       if (span_of(a.b, a.c.ps, s).bad) set_status(a.status, UWC_DEV_RANGE);
   const Part part = find_part(a);
@@ -173,8 +176,10 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
     int it = 0;
     int s = part.seq, h = part.head, t0 = part.tile;
     long long left = part.count;
+#pragma unroll 1
     while (left > 0) {
       const Unit k = unit_of(a, s);
+#pragma unroll 1
       for (; h < Hkv && t0 < k.total && left > 0;) {
         const int end = (int)min((long long)k.total, t0 + left);
         // page ids and scales of eight tiles, one 16-key group a lane
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           page = -1;
           sc = make_float2(0.f, 0.f);
           if (i < end && k.seen(j0, 16)) {
-            page = page_at(a.b, a.c, s, j0 / ps);
+            page = page_at(a.b, a.c, s, j0 >> a.c.lg);
             if (page < 0) set_status(a.status, UWC_DEV_RANGE);
             else sc = make_float2(a.c.sk[(size_t)page * Hkv + h], a.c.sv[(size_t)page * Hkv + h]);
           }
@@ -192,14 +197,18 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
         int page, j0, npage = -1, nj0 = 0;
         float2 sc, nsc = make_float2(0.f, 0.f);
         fetch(t0, page, sc, j0);
+#pragma unroll 1
         for (int tb = t0; tb < end; tb += kBatch) {
           if (tb + kBatch < end) fetch(tb + kBatch, npage, nsc, nj0);
+#pragma unroll 1
           for (int i = 0; i < kBatch && tb + i < end; i++, it++) {
             const int st = it % ST;
             const uint32_t use = (uint32_t)(it / ST);
             if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[st], (use - 1) & 1, &s_abort, a.status))) {
               // give up: let the copies in flight land (bounded), then leave
+#pragma unroll 1
               for (int x = max(0, it - ST); x < it; x++)
+#pragma unroll 1
                 for (int n = 0; n < (1 << 16) && !mbar_try_wait(&full[x % ST], (uint32_t)(x / ST) & 1); n++) {
                 }
               return;
@@ -220,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
             if (elect_one()) mbar_expect_tx(&full[st], (uint32_t)(boxes * 2 * box * kHd));
             __syncwarp();
             if (issue) {
-              const int y = (bpage * Hkv + h) * ps + j0 % ps;
+              const int y = (bpage * Hkv + h) * ps + (j0 & (ps - 1));
               uint8_t* dst = sm + st * kStageBytes + grp * 16 * kHd;
               tma_load_2d(dst, &mapK, &full[st], 0, y);
               tma_load_2d(dst + kTile * kHd, &mapV, &full[st], 0, y);
@@ -241,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
       s++;
       h = 0;
       t0 = 0;
+#pragma unroll 1
       while (left > 0 && s < a.b.seqs && unit_of(a, s).total == 0) s++;
       if (s >= a.b.seqs) break;
     }
@@ -257,9 +267,11 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
   int it = 0;
   int s = part.seq, h = part.head, t0 = part.tile;
   long long left = part.count, at = part.first;      // at: the line's tile that t0 is
+#pragma unroll 1
   while (left > 0) {
     const Unit k = unit_of(a, s);
     const int rows = k.sp.n * G;
+#pragma unroll 1
     for (; h < Hkv && left > 0; h++, t0 = 0) {
       const int end = (int)min((long long)k.total, t0 + left);
       // ---- this unit's queries: row r = token r / G, head r % G; thread (g, t) has dims 32 t .. of rows g + 8 n
@@ -321,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           for (int j = 0; j < 4; j++) o[n][i][j] = 0.f;
       }
       // ---- the tiles
+#pragma unroll 1
       for (int i = t0; i < end; i++, it++) {
         const int st = it % ST;
         // after a wait that ran out the warps run through their schedule without computing
@@ -547,9 +560,11 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
         if (s_last) {
           const int b0 = (int)(u0 / part.per), b1 = (int)((u0 + k.total - 1) / part.per);
           __threadfence();
+#pragma unroll 1
           for (int r = warp; r < rows; r += kWarps) {
             auto slot = [&](int b) { return (size_t)(2 * b + (b == b0)) * R + r; };
             float M = kNoMax, L = 0.f;
+#pragma unroll 1
             for (int b = b0 + lane; b <= b1; b += 32) M = fmaxf(M, __ldcg(&ta.part_ml[slot(b)]).x);
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
@@ -578,6 +593,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
     s++;
     h = 0;
     t0 = 0;
+#pragma unroll 1
     while (left > 0 && s < a.b.seqs && unit_of(a, s).total == 0) s++;
     if (s >= a.b.seqs) break;
   }
@@ -658,7 +674,7 @@ extern "C" int uwc_paged_attention(const int8_t* kc, const float* sk, const int8
                                    int sinks, void* workspace, uint64_t workspace_bytes, void* stream) {
   AttnArgs a = {};
   a.c = Cache{const_cast<int8_t*>(kc), const_cast<float*>(sk), const_cast<int8_t*>(vc), const_cast<float*>(sv), pages,
-              page_size, Hkv};
+              page_size, Hkv, 0};
   a.b = Seqs{table, start, cu, seqs, width, rows, max_new};
   const int rc = uwc_paged_check(&a.c, &a.b);
   if (rc != UWC_OK) return rc;

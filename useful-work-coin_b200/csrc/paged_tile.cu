@@ -4,15 +4,17 @@
 // k_paged_tile: an item is 256 rows of one (sequence, KV head) -- its tokens times the query heads of the
 // group, token-major, so every head of the group uses a key tile once -- as two 128-row tiles. The bound is
 // the tensor core (S = Q K^T and O = P V, tcgen05 kind::f16) against the exponentials (one each score).
-// Roles of a CTA (one per SM, 13 warps):
+// Roles of a CTA (one per SM, 16 warps; registers go from the others to the softmax):
 //   warps 0-3, 4-7   the softmax of the first and second 128 rows, a row a thread: scores from TMEM, the
 //                    running maximum and sum in float32 registers, weights back to TMEM as fp16 over the
 //                    scores that they came from. They also turn the queries to fp16 and write the output.
-//   warps 8-11       pages to operands: 128 keys of int8 from HBM through registers to fp16 in shared memory
-//                    (the integers are exact; a byte permute and a subtraction a pair), two stages each for
-//                    keys and values, so no scale is multiplied in: the key scale multiplies the score, the
-//                    value scale (over a reference that follows its size) the weight, both a page's constant.
+//   warps 8-11       pages to operands: 128 keys of int8 from HBM through registers (a tile ahead) to fp16
+//                    in shared memory (the integers are exact; a byte permute and a subtraction a pair), two
+//                    stages each for keys and values. No scale is multiplied in: the key scale multiplies the
+//                    score, the value scale (over a reference that follows its size) the weight.
 //   warp 12          one thread issues the products: while one row tile is in its softmax the other's run.
+//   warp 13          walks the line (below) and hands the pieces to the others.
+//   warp 14          looks the tiles' pages and their scales up, up to four tiles ahead.
 // O stays in TMEM; it is rescaled only when a row's maximum grew by more than 2^4 (so a weight is
 // below 1024 * 2^4 * 2 in fp16, and keeps its 11 bits down to 2^-24 of the reference) or the tile's largest value
 // scale left [1/64, 2] of the reference; both are rare after an item's first tile.
@@ -31,10 +33,11 @@ using namespace paged;
 constexpr int kRows = 128;                   // rows of a softmax warpgroup
 constexpr int kTile = 128;                   // keys per tile
 constexpr int kGroups = kTile / 16;          // 16-key groups, each inside one page
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;            // the last warp only gives its registers up
 constexpr int kHalf = kTile * 128;           // bytes of 128 rows x 64 dims of fp16 (one swizzled block)
 constexpr int kOperand = 2 * kHalf;          // a 128 x 128 fp16 operand
-constexpr int kScaleRing = 4;
+constexpr int kAhead = 4;                    // tiles whose pages are looked up ahead of their loads
+constexpr int kPageRing = 8;                 // slots: those, and up to four that the softmax still reads scales of
 constexpr int kSeqs = 1024;                  // sequences whose span and tiles are kept in shared memory
 constexpr int kSmem = 1024 + 6 * kOperand + kSeqs * 24;   // two query tiles, two stages of keys, two of values
 constexpr int kMinTiles = 4;                 // a CTA's least share of the line
@@ -45,7 +48,7 @@ constexpr float kWeightUnit = 1024.f;         // the fp16 weight of p = 1 at the
 
 struct TileArgs {
   AttnArgs a;
-  float* part_o;           // (2 grid, 256, 128): a CTA's two partial items, unnormalized
+  float* part_o;           // (2 grid, 2, 32, 128, 4): a CTA's two partial items by row tile, four columns, row; unnormalized
   float2* part_ml;         // (2 grid, 256): running maximum (log2), sum
   uint32_t* counters;      // (grid, 2): finished parts of the item that starts in this CTA; left zero
 };
@@ -73,21 +76,25 @@ struct Batch {
   __device__ __forceinline__ long long count(const Span& z) const {
     const int nb = blocks(z);
     long long t = 0;
+#pragma unroll 1
     for (int b = threadIdx.x & 31; b < nb; b += 32) t += Item(a, z, G, b).total;
     return warp_sumll(t);
   }
   __device__ __forceinline__ long long tiles(int s) const { return s < kSeqs ? tiles_[s] : count(span(s)); }
   __device__ __forceinline__ void load() {
     const int n = min(a.b.seqs, kSeqs);
+#pragma unroll 1
     for (int s = threadIdx.x; s < n; s += kThreads) {
       const Span z = span_of(a.b, a.c.ps, s);
       if (z.bad && blockIdx.x == 0) set_status(a.status, UWC_DEV_RANGE);
       span_[s] = make_int4(z.row0, z.n, z.start, z.idle);
     }
     if (blockIdx.x == 0)
+#pragma unroll 1
       for (int s = kSeqs + threadIdx.x; s < a.b.seqs; s += kThreads)
         if (span_of(a.b, a.c.ps, s).bad) set_status(a.status, UWC_DEV_RANGE);
     __syncthreads();
+#pragma unroll 1
     for (int s = threadIdx.x / 32; s < n; s += kThreads / 32) {
       const long long t = count(span(s));
       if ((threadIdx.x & 31) == 0) tiles_[s] = t;
@@ -95,41 +102,38 @@ struct Batch {
   }
 };
 
-// A CTA's walk along the line: pieces (sequence, KV head, block, tiles t0 .. t1 - 1). Every warp walks for
-// itself, all lanes together.
-struct Walk {
-  const Batch& q;
-  const AttnArgs& a;
-  int G, s, h, blk, blks;
-  int t0, t1, total;       // this piece's tiles, the item's
-  long long at, left, per; // the line's tile that t0 is; tiles of this CTA from t0 on
-  Span sp;
-
-  __device__ __forceinline__ Walk(const Batch& batch) : q(batch), a(batch.a), G(batch.G) {
-    const int lane = threadIdx.x & 31, S = a.b.seqs, kept = min(S, kSeqs);
-    long long sum = 0;
-    for (int i = lane; i < kept; i += 32) sum += q.tiles(i);
-    sum = warp_sumll(sum);
-    for (int i = kept; i < S; i++) sum += q.tiles(i);
-    sum *= a.c.Hkv;
-    per = max((sum + gridDim.x - 1) / gridDim.x, (long long)kMinTiles);
-    at = per * blockIdx.x;
-    left = min(per, sum - at);
-    if (left <= 0) return;
-    // the sequence, then the block, that tile `at` lies in
-    long long rest = at;
-    for (s = 0; s < S; s++) {
-      const long long one = q.tiles(s);
-      if (rest >= one * a.c.Hkv) {
-        rest -= one * a.c.Hkv;
-        continue;
-      }
-      sp = q.span(s);
-      blks = q.blocks(sp);
-      h = (int)(rest / one);
-      rest %= one;
+// A CTA's part of the line of key tiles: `left` tiles from tile t0 of block blk of KV head h of sequence s on.
+struct Start {
+  int s, h, blk, t0;
+  int left, per;
+};
+// One warp, all lanes together.
+__device__ __forceinline__ Start find_start(const Batch& q) {
+  const int lane = threadIdx.x & 31, S = q.a.b.seqs, kept = min(S, kSeqs), Hkv = q.a.c.Hkv;
+  long long sum = 0;
+#pragma unroll 1
+  for (int i = lane; i < kept; i += 32) sum += q.tiles_[i];
+  sum = warp_sumll(sum);
+#pragma unroll 1
+  for (int i = kept; i < S; i++) sum += q.tiles(i);
+  sum *= Hkv;
+  Start p = {};
+  // no less than an even share (a division of 64 bits is long code): grid * per >= sum
+  p.per = max(kMinTiles, (int)((float)sum / (float)gridDim.x * 1.000001f) + 1);
+  long long rest = (long long)p.per * blockIdx.x;
+  p.left = (int)max(0ll, min((long long)p.per, sum - rest));
+  if (p.left == 0) return p;
+#pragma unroll 1
+  for (; p.s < S; p.s++) {
+    const long long one = q.tiles(p.s);
+    if (rest < one * Hkv) {
+      const Span sp = q.span(p.s);
+      const int blks = q.blocks(sp);
+#pragma unroll 1
+      for (; rest >= one; p.h++) rest -= one;
+#pragma unroll 1
       for (int b0 = 0; b0 < blks; b0 += 32) {
-        const int t = b0 + lane < blks ? Item(a, sp, G, b0 + lane).total : 0;
+        const int t = b0 + lane < blks ? Item(q.a, sp, q.G, b0 + lane).total : 0;
         int inc = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -139,43 +143,31 @@ struct Walk {
         const unsigned hit = __ballot_sync(0xffffffffu, inc > rest);
         if (hit) {
           const int l = __ffs(hit) - 1;
-          blk = b0 + l;
-          t0 = (int)(rest - __shfl_sync(0xffffffffu, inc - t, l));
-          break;
+          p.blk = b0 + l;
+          p.t0 = (int)(rest - __shfl_sync(0xffffffffu, inc - t, l));
+          return p;
         }
         rest -= __shfl_sync(0xffffffffu, inc, 31);
       }
-      break;
     }
-    piece();
+    rest -= one * Hkv;
   }
-  __device__ __forceinline__ void piece() {
-    total = Item(a, sp, G, blk).total;
-    t1 = (int)min((long long)total, t0 + left);
-  }
-  __device__ __forceinline__ bool more() const { return left > 0; }
-  __device__ __forceinline__ void next() {
-    at += t1 - t0;
-    left -= t1 - t0;
-    if (left <= 0) return;
-    t0 = 0;
-    if (++blk == blks) {
-      blk = 0;
-      if (++h == a.c.Hkv) {
-        h = 0;
-        do {
-          sp = q.span(++s);
-          blks = q.blocks(sp);
-        } while (blks == 0 && s + 1 < a.b.seqs);
-      }
-    }
-    piece();
-  }
-  __device__ __forceinline__ int rows(int w) const { return min(kRows, max(0, sp.n * G - 2 * kRows * blk - kRows * w)); }
-  // the CTAs that the item's parts lie in
-  __device__ __forceinline__ int first_cta() const { return (int)((at - t0) / per); }
-  __device__ __forceinline__ int last_cta() const { return (int)((at - t0 + total - 1) / per); }
+  p.left = 0;
+  return p;
+}
+
+// One piece of it, inside one item, as the roles read it from shared memory.
+struct Piece {
+  int rows;                // rows of the item (0 ends the CTA's work), the first kRows of them warpgroup 0's
+  int row0, first;         // the sequence's first row of the row tensors, the item's first row of the sequence
+  int seq, head, start;    // start: -1 where the slot is idle
+  int t0, t1, whole;       // tiles; whether they are the whole item
+  int b0, b1;              // the CTAs that have parts of it
+  int lo, hi, sink_end, tA, tB0;
+  __device__ __forceinline__ int key(int i) const { return (i < tA ? i : tB0 + (i - tA)) * kTile; }
+  __device__ __forceinline__ bool seen(int j, int n) const { return j < sink_end || (j < hi && j + n > lo); }
 };
+constexpr int kPieces = 4;   // pieces known ahead
 
 // ---- tcgen05
 __device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr) {
@@ -213,13 +205,61 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 struct Bars {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], wg[2], fin;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
 };
 
-// Ends the role when a wait ran out (the status is set, the other roles follow by the abort flag).
+// Pairs of float32 (one instruction for two), and the larger of three.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float lo_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+  return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c));
+}
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) { return max3(a, __uint_as_float(b), __uint_as_float(c)); }
+
+// Ends the role when a wait ran out; the other roles' waits then run out too.
 #define TILE_WAIT(bar, parity) \
-  if (!__all_sync(0xffffffffu, mbar_wait(&(bar), (parity), &s_abort, a.status))) goto done
+  if (!warp_wait(&(bar), (parity))) goto timeout
+
+// A role's next piece, and its place in the ring given back.
+#define TILE_PIECE(n)                                                                        \
+  TILE_WAIT(bar.piece_full[(n) % kPieces], ((n) / kPieces) & 1);                             \
+  const Piece& k = s_piece[(n) % kPieces];                                                   \
+  if (k.rows == 0) break
+#define TILE_PIECE_DONE(n)                                                                   \
+  __syncwarp();                                                                              \
+  if (lane == 0) mbar_arrive(&bar.piece_empty[(n) % kPieces])
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
@@ -227,25 +267,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   extern __shared__ uint8_t sm_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bar;
-  __shared__ float2 s_scale[kScaleRing][kGroups];   // key scale (-1: no key of the group is seen), value scale
+  __shared__ Piece s_piece[kPieces];
+  __shared__ __align__(16) float2 s_scale[kPageRing][kGroups];   // key scale (-1: no key of the group is seen), value scale
+  __shared__ int s_row[kPageRing][kGroups];        // first cache row of the group's keys (-1: none; -2: no more tiles)
+  __shared__ Start s_start;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_last[2];
+  __shared__ int s_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smQ = smem_u32(sm), smK = smQ + 2 * kOperand, smV = smK + 2 * kOperand;
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(&bar.q_full[i], kRows);
-      mbar_init(&bar.k_full[i], 128);
+      mbar_init(&bar.q_full[i], 4);
+      mbar_init(&bar.k_full[i], 4);
       mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_full[i], 128);
+      mbar_init(&bar.v_full[i], 4);
       mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.s_full[i], 2);
-      mbar_init(&bar.p_full[i], kRows);
+      mbar_init(&bar.p_full[i][0], 4);
+      mbar_init(&bar.p_full[i][1], 4);
       mbar_init(&bar.o_done[i], 1);
-      mbar_init(&bar.wg[i], kRows);
+      mbar_init(&bar.wg[i], 4);
     }
     mbar_init(&bar.fin, 1);
-    s_abort = 0;
+    for (int i = 0; i < kPieces; i++) {
+      mbar_init(&bar.piece_full[i], 1);
+      mbar_init(&bar.piece_empty[i], 10);
+    }
+    for (int i = 0; i < kAhead; i++) {
+      mbar_init(&bar.page_full[i], 1);
+      mbar_init(&bar.page_empty[i], 4);
+    }
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -255,40 +306,67 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   Batch batch{a, a.H / a.c.Hkv, reinterpret_cast<int4*>(sm + 6 * kOperand),
               reinterpret_cast<long long*>(sm + 6 * kOperand + kSeqs * 16)};
   batch.load();
+  __syncthreads();
+  if (warp == 0) {
+    const Start p = find_start(batch);
+    if (lane == 0) s_start = p;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int Hkv = a.c.Hkv, ps = a.c.ps;
+  const int Hkv = a.c.Hkv, ps = a.c.ps, G = a.H / Hkv;
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ------------------------------------------------------------------ softmax, a row a thread
     const int w = warp >> 2, r = tid & (kRows - 1);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
+    const float inv_g = 1.0f / (float)G;
     uint32_t it = 0, all = 0, wgp = 0;             // this warpgroup's tiles, every tile, its barrier's phases
-    for (Walk k(batch); k.more(); k.next()) {
-      const int rows = k.rows(w);
-      if (rows == 0) {                             // only w = 1: the second tile of a short block
+#pragma unroll 1
+    for (uint32_t n = 0;; n++) {
+      TILE_PIECE(n);
+      const int rows = min(kRows, k.rows - kRows * w);
+      if (rows <= 0) {                             // only w = 1: the second tile of a short item
         all += k.t1 - k.t0;
+        TILE_PIECE_DONE(n);
         continue;
       }
-      const int row = 2 * kRows * k.blk + kRows * w + r, t = row / k.G, hh = k.h * k.G + row % k.G;
+      // row x of the item is token tok0 + (x + rem0) / G of the sequence: a division of small numbers, exact in
+      // float32 while they are below 2^20. A lane keeps its own row's (token - tok0, head of the group).
+      const int tok0 = k.first / G, rem0 = k.first - tok0 * G;
+      auto token_of = [&](int x) { return (int)(((float)(x + rem0) + 0.5f) * inv_g); };
+      const int my_tok = token_of(kRows * w + r), my_head = kRows * w + r + rem0 - my_tok * G;
       const bool live = r < rows;
-      const int pos = live && !k.sp.idle ? k.sp.start + t : -1;
-      const Item key(a, k.sp, k.G, k.blk);
-      // ---- the query row as fp16 (its largest value at 2^14), into the swizzled operand
+      const int pos = live && k.start >= 0 ? k.start + tok0 + my_tok : -1;
+      // ---- the query rows, two a warp at a time, into their places in the swizzled operand, ...
+      {
+        const int c = lane & 15;
+        const T* q = reinterpret_cast<const T*>(a.q) + (long long)(k.row0 + tok0) * a.q_tok + (long long)(k.head * G) * a.q_head + 8 * c;
+        const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf;
+#pragma unroll 2
+        for (int i = 0; i < 16; i++) {
+          const int x = 2 * i + (lane >> 4), rr = 32 * (warp & 3) + x;
+          const int tk = __shfl_sync(0xffffffffu, my_tok, x), hd = __shfl_sync(0xffffffffu, my_head, x);
+          const uint32_t dst = at + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(rr < rows ? q + tk * a.q_tok + hd * a.q_head : q),
+                       "r"(rr < rows ? 16 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+      }
+      // ... where each thread turns its own row to fp16, its largest value at 2^14
       float qmul;
       {
-        uint4 x[16];
-        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (long long)(k.sp.row0 + t) * a.q_tok +
-                                                        (long long)hh * a.q_head);
+        const uint32_t at = smQ + w * kOperand + r * 128;
         float mx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = live ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < 16; i++) {
-          const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          const uint4 x = lds128(at + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4));
+          const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const float2 f = two_f(u[j], T());
@@ -298,62 +376,91 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         const int e = row_exponent(mx);
         const float up = a.scale < 0.f ? -pow2i(e) : pow2i(e);   // a negative scale goes with the query
         qmul = fabsf(a.scale) * kLog2OfE * pow2i(-e);
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < 16; i++) {
-          uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          const uint32_t place = at + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4);
+          const uint4 x = lds128(place);
+          uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const float2 f = two_f(u[j], T());
             u[j] = pack2(f.x * up, f.y * up, __half());
           }
-          sts128(smQ + w * kOperand + (i >> 3) * kHalf + r * 128 + (((i & 7) ^ (r & 7)) << 4), make_uint4(u[0], u[1], u[2], u[3]));
+          sts128(place, make_uint4(u[0], u[1], u[2], u[3]));
         }
       }
       fence_async_smem();
-      mbar_arrive(&bar.q_full[w]);
+      warp_arrive(&bar.q_full[w]);
       // positions of this warpgroup's first and last row bound where its masks are needed
-      const int pa = k.sp.idle ? -1 : k.sp.start + (2 * kRows * k.blk + kRows * w) / k.G;
-      const int pb = k.sp.idle ? -1 : k.sp.start + (2 * kRows * k.blk + kRows * w + rows - 1) / k.G;
+      const int pa = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w);
+      const int pb = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rows - 1);
       float m = kNoMax, l = 0.f, ref = 0.f;
+#pragma unroll 1
       for (int i = k.t0; i < k.t1; i++, it++, all++) {
-        const int j0 = key.key(i);
+        const int j0 = k.key(i);
         TILE_WAIT(bar.s_full[w], it & 1);
         tc_fence_after();
-        const float2* sc = s_scale[all % kScaleRing];
-        bool seen = true;
-        float f[kGroups], vs = 0.f;
+        const float2* sc = s_scale[all % kPageRing];
+        uint32_t s0[32], s1[32];
+        auto load = [&](int c, uint32_t* s) { tmem_ld_32x32b_x32(tS + 32 * c, s); };
+        // whether some key is hidden from some row: past its position, out of its window, without a page
+        bool hidden = j0 + kTile - 1 > pa || (a.window >= 0 && !(j0 > pb - a.window || j0 + kTile <= a.sinks));
+        float kf[kGroups], vf[kGroups], vs = 0.f;
+#pragma unroll
+        for (int g = 0; g < kGroups; g += 2) {
+          const uint4 x = lds128(smem_u32(sc + g));
+          kf[g] = __uint_as_float(x.x);
+          vf[g] = __uint_as_float(x.y);
+          kf[g + 1] = __uint_as_float(x.z);
+          vf[g + 1] = __uint_as_float(x.w);
+        }
 #pragma unroll
         for (int g = 0; g < kGroups; g++) {
-          const float2 x = sc[g];
-          seen &= x.x >= 0.f;
-          f[g] = fmaxf(x.x * qmul, 1e-37f);        // not 0: a hidden score stays -inf
-          vs = fmaxf(vs, x.y);
+          hidden |= kf[g] < 0.f;
+          vs = fmaxf(vs, vf[g]);
+          kf[g] = fmaxf(kf[g] * qmul, 1e-37f);     // a page's factor for scores (log2); not 0: a hidden score stays -inf
         }
-        const bool masked = !seen || !(j0 + kTile - 1 <= pa && (a.window < 0 || j0 > pb - a.window || j0 + kTile <= a.sinks));
-        auto load = [&](int c, uint32_t* s) {      // 64 scores of this row, hidden ones -inf
-          tmem_ld_32x32b_x32(tS + 64 * c, s);
-          tmem_ld_32x32b_x32(tS + 64 * c + 32, s + 32);
-          tmem_wait_ld();
-          if (masked) {
+        if (hidden) {
+          // only tiles at an edge: their hidden scores become -inf where they are, in a rolled loop (the code
+          // around it is straight-line, and every instruction of it is fetched for every tile)
+#pragma unroll 1
+          for (int c = 0; c < 4; c++) {
+            load(c, s0);
+            tmem_wait_ld();
+            const int last = pos - j0 - 32 * c, from = a.window < 0 ? -kTile : last - a.window, sink = a.sinks - j0 - 32 * c;
+            const bool g0 = sc[2 * c].x < 0.f, g1 = sc[2 * c + 1].x < 0.f;
 #pragma unroll
-            for (int x = 0; x < 64; x++) {
-              const int j = j0 + 64 * c + x;
-              if (!sees(a, pos, j) || sc[4 * c + x / 16].x < 0.f) s[x] = 0xff800000u;
-            }
+            for (int x = 0; x < 32; x++)
+              s0[x] = x > last || (x <= from && x >= sink) || (x < 16 ? g0 : g1) ? 0xff800000u : s0[x];
+            tmem_st_32x32b_x32(tS + 32 * c, s0);
+          }
+          tmem_wait_st();
+        }
+        float mx = kNoMax;
+        auto top = [&](const uint32_t* s, float f0, float f1) {
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const uint32_t* z = s + 16 * g;
+            float u = max3(z[0], z[1], z[2]), v = max3(z[3], z[4], z[5]);
+            u = max3(u, z[6], z[7]);
+            v = max3(v, z[8], z[9]);
+            u = max3(u, z[10], z[11]);
+            v = max3(v, z[12], z[13]);
+            u = max3(u, z[14], z[15]);
+            mx = fmaxf(mx, fmaxf(u, v) * (g ? f1 : f0));
           }
         };
-        uint32_t s[64];
-        float mx = kNoMax;
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          load(c, s);
-#pragma unroll
-          for (int g = 0; g < 4; g++) {
-            float x = __uint_as_float(s[16 * g]);
-#pragma unroll
-            for (int y = 1; y < 16; y++) x = fmaxf(x, __uint_as_float(s[16 * g + y]));
-            mx = fmaxf(mx, x * f[4 * c + g]);
-          }
+        // 32 columns at a time, the next ones on their way. Rolled: the straight-line form needs 11 KB of
+        // instructions for every tile, and waits for them
+        load(0, s0);
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_wait_ld();
+          load(c + 1, s1);
+          top(s0, c ? kf[4] : kf[0], c ? kf[5] : kf[1]);
+          tmem_wait_ld();
+          load(2, s0);
+          top(s1, c ? kf[6] : kf[2], c ? kf[7] : kf[3]);
         }
         // ---- raise the maximum or the value reference, and bring O along (its products must be done)
         const bool raise = mx > m + kRaise, refer = vs > 2.f * ref || (vs > 0.f && vs < ref * (1.f / 64.f));
@@ -367,253 +474,426 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           if (i > k.t0) {
             TILE_WAIT(bar.o_done[w], (it - 1) & 1);
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-              tmem_ld_32x32b_x32(tO + 32 * c, s);
+#pragma unroll 1
+            for (int c = 0; c < 8; c++) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(tO + 16 * c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 32; x++) s[x] = __float_as_uint(__uint_as_float(s[x]) * by);
-              tmem_st_32x32b_x32(tO + 32 * c, s);
+              for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * by);
+              tmem_st_32x32b_x16(tO + 16 * c, o);
             }
           }
         }
-        // ---- weights: p = 2^(score - m); the row sum keeps p, the product gets p s_v / ref in fp16
+        // ---- weights: p = 2^(score - m); the row sum keeps p, the product gets p s_v / ref in fp16. The
+        // last 64 keys' product starts while the others' weights are computed.
         const float unit = ref > 0.f ? __fdividef(kWeightUnit, ref) : 0.f;
+        const uint64_t nm = two(-m, -m);
+        uint64_t l2[2] = {0ull, 0ull};
+        uint32_t p[32];
+        auto weigh = [&](const uint32_t* s, uint32_t* to, float f0, float f1, float w0, float w1) {
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-          load(c, s);
-          uint32_t p[32];
-#pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const float fg = f[4 * c + g], wg = sc[4 * c + g].y * unit;
+          for (int g = 0; g < 2; g++) {
+            const float fg = g ? f1 : f0, wg = (g ? w1 : w0) * unit;
+            const uint64_t fg2 = two(fg, fg), wg2 = two(wg, wg);
 #pragma unroll
             for (int y = 0; y < 8; y++) {
-              const float x0 = exp2_fast(fmaf(__uint_as_float(s[16 * g + 2 * y]), fg, -m));
-              const float x1 = exp2_fast(fmaf(__uint_as_float(s[16 * g + 2 * y + 1]), fg, -m));
-              l += x0 + x1;
-              p[8 * g + y] = pack2(x0 * wg, x1 * wg, __half());
+              const int x = 16 * g + 2 * y;
+              const uint64_t z = fma2(two(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), fg2, nm);
+              const uint64_t e = two(exp2_fast(lo_of(z)), exp2_fast(hi_of(z)));
+              l2[y & 1] = add2(l2[y & 1], e);
+              const uint64_t q = mul2(e, wg2);
+              to[8 * g + y] = pack2(lo_of(q), hi_of(q), __half());
             }
           }
-          tmem_st_32x32b_x16(tS + 32 * c, p);
-          tmem_st_32x32b_x16(tS + 32 * c + 16, p + 16);
+        };
+        // keys 64 .. 127 first, over their own scores, then keys 0 .. 63
+#pragma unroll 1
+        for (int h = 1; h >= 0; h--) {
+          tmem_wait_ld();
+          load(2 * h + 1, s1);
+          weigh(s0, p, h ? kf[4] : kf[0], h ? kf[5] : kf[1], h ? vf[4] : vf[0], h ? vf[5] : vf[1]);
+          tmem_wait_ld();
+          if (h) load(0, s0);
+          weigh(s1, p + 16, h ? kf[6] : kf[2], h ? kf[7] : kf[3], h ? vf[6] : vf[2], h ? vf[7] : vf[3]);
+          tmem_st_32x32b_x32(tS + 64 * h, p);
+          tmem_wait_st();
+          tc_fence_before();
+          warp_arrive(&bar.p_full[w][h]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bar.p_full[w]);
+        l += (lo_of(l2[0]) + hi_of(l2[0])) + (lo_of(l2[1]) + hi_of(l2[1]));
       }
       // ---- the item's (or the part's) result
       TILE_WAIT(bar.o_done[w], (it - 1) & 1);
       tc_fence_after();
-      const bool whole = k.t0 == 0 && k.t1 == k.total;
       const float back = ref * (1.f / kWeightUnit);
-      T* out = reinterpret_cast<T*>(a.out) + ((size_t)(k.sp.row0 + t) * a.H + hh) * kHd;
-      if (whole) {
-        const float inv = l == 0.f ? 0.f : back / l;
+      // through this warp's rows of the (idle) query operand, so that a row of the output leaves in one piece
+      auto store = [&](int c, const float* o, float f) {             // 32 columns
+        const uint32_t at = smQ + w * kOperand + (c >> 1) * kHalf + r * 128;
 #pragma unroll
+        for (int x = 0; x < 4; x++)
+          sts128(at + (((4 * (c & 1) + x) ^ (r & 7)) << 4),
+                 make_uint4(pack2(o[8 * x] * f, o[8 * x + 1] * f, T()), pack2(o[8 * x + 2] * f, o[8 * x + 3] * f, T()),
+                            pack2(o[8 * x + 4] * f, o[8 * x + 5] * f, T()), pack2(o[8 * x + 6] * f, o[8 * x + 7] * f, T())));
+      };
+      auto flush = [&]() {
+        __syncwarp();
+        const int c = lane & 15;
+        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((size_t)(k.row0 + tok0) * a.H + k.head * G) * kHd) + c;
+        const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf;
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) {
+          const int x = 2 * i + (lane >> 4), rr = 32 * (warp & 3) + x;
+          const int row = __shfl_sync(0xffffffffu, my_tok * a.H + my_head, x);   // of the item's first token's
+          const uint4 v = lds128(at + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+          if (rr < rows) out[(long long)row * (kHd / 8)] = v;
+        }
+        __syncwarp();
+      };
+      if (k.whole) {
+        const float inv = l == 0.f ? 0.f : back / l;
+#pragma unroll 1
         for (int c = 0; c < 4; c++) {
           uint32_t s[32];
           tmem_ld_32x32b_x32(tO + 32 * c, s);
           tmem_wait_ld();
-          if (live) {
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-              uint32_t u[4];
-#pragma unroll
-              for (int y = 0; y < 4; y++)
-                u[y] = pack2(__uint_as_float(s[8 * x + 2 * y]) * inv, __uint_as_float(s[8 * x + 2 * y + 1]) * inv, T());
-              reinterpret_cast<uint4*>(out + 32 * c)[x] = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
+          store(c, reinterpret_cast<const float*>(s), inv);
         }
         tc_fence_before();
+        flush();
+        TILE_PIECE_DONE(n);
         continue;
       }
-      const int b0 = k.first_cta(), b1 = k.last_cta();
-      {
-        const size_t slot = ((size_t)(2 * blockIdx.x + (k.t0 == 0)) * 2 + w) * kRows + r;
+      // a part: its O column-major (four columns of a row together), which its own thread of the joining
+      // CTA reads back the same way
+      const int b0 = k.b0, b1 = k.b1;
+      auto part_o = [&](int b) { return reinterpret_cast<float4*>(ta.part_o) + ((size_t)(2 * b + (b == b0)) * 2 + w) * 32 * kRows + r; };
+      auto part_ml = [&](int b) { return ta.part_ml + ((size_t)(2 * b + (b == b0)) * 2 + w) * kRows + r; };
+#pragma unroll 1
+      for (int c = 0; c < 4; c++) {
+        uint32_t s[32];
+        tmem_ld_32x32b_x32(tO + 32 * c, s);
+        tmem_wait_ld();
+        float4* po = part_o(blockIdx.x) + 8 * c * kRows;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(tO + 32 * c, s);
-          tmem_wait_ld();
-          if (live) {
-            float4* po = reinterpret_cast<float4*>(ta.part_o + slot * kHd + 32 * c);
-#pragma unroll
-            for (int x = 0; x < 8; x++)
-              po[x] = make_float4(__uint_as_float(s[4 * x]) * back, __uint_as_float(s[4 * x + 1]) * back,
-                                  __uint_as_float(s[4 * x + 2]) * back, __uint_as_float(s[4 * x + 3]) * back);
-          }
-        }
-        if (live) ta.part_ml[slot] = make_float2(m, l);
-        tc_fence_before();
+        for (int x = 0; x < 8; x++)
+          po[x * kRows] = make_float4(__uint_as_float(s[4 * x]) * back, __uint_as_float(s[4 * x + 1]) * back,
+                                      __uint_as_float(s[4 * x + 2]) * back, __uint_as_float(s[4 * x + 3]) * back);
       }
+      *part_ml(blockIdx.x) = make_float2(m, l);
+      tc_fence_before();
       __threadfence();
-      mbar_arrive(&bar.wg[w]);
+      warp_arrive(&bar.wg[w]);
       TILE_WAIT(bar.wg[w], wgp & 1);
       wgp++;
       if (r == 0) {
-        const uint32_t n = atomicAdd(&ta.counters[2 * b0 + w], 1u);
-        s_last[w] = n == (uint32_t)(b1 - b0);
+        const uint32_t arrived = atomicAdd(&ta.counters[2 * b0 + w], 1u);
+        s_last[w] = arrived == (uint32_t)(b1 - b0);
         if (s_last[w]) ta.counters[2 * b0 + w] = 0;
         __threadfence();
       }
-      mbar_arrive(&bar.wg[w]);
+      warp_arrive(&bar.wg[w]);
       TILE_WAIT(bar.wg[w], wgp & 1);
       wgp++;
-      if (s_last[w] && live) {
+      if (s_last[w]) {
         __threadfence();
-        auto slot = [&](int b) { return ((size_t)(2 * b + (b == b0)) * 2 + w) * kRows + r; };
         float M = kNoMax, L = 0.f;
-        for (int b = b0; b <= b1; b++) M = fmaxf(M, __ldcg(&ta.part_ml[slot(b)]).x);
+#pragma unroll 1
+        for (int b = b0; b <= b1; b++) M = fmaxf(M, __ldcg(part_ml(b)).x);
+#pragma unroll 1
         for (int b = b0; b <= b1; b++) {
-          const float2 ml = __ldcg(&ta.part_ml[slot(b)]);
+          const float2 ml = __ldcg(part_ml(b));
           L = fmaf(ml.y, exp2_fast(ml.x - M), L);
         }
         const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll 1
-        for (int c = 0; c < 16; c++) {
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        for (int c = 0; c < 4; c++) {
+          float o[32];
+#pragma unroll
+          for (int x = 0; x < 32; x++) o[x] = 0.f;
+          float4 u[8];
+          auto read = [&](int b) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) u[x] = __ldcg(part_o(b) + (8 * c + x) * kRows);
+          };
+          read(b0);
+#pragma unroll 1
           for (int b = b0; b <= b1; b++) {
-            const float f = exp2_fast(__ldcg(&ta.part_ml[slot(b)]).x - M);
-            const float4* po = reinterpret_cast<const float4*>(ta.part_o + slot(b) * kHd) + 2 * c;
-            const float4 u = __ldcg(po), v = __ldcg(po + 1);
-            x = make_float4(fmaf(u.x, f, x.x), fmaf(u.y, f, x.y), fmaf(u.z, f, x.z), fmaf(u.w, f, x.w));
-            y = make_float4(fmaf(v.x, f, y.x), fmaf(v.y, f, y.y), fmaf(v.z, f, y.z), fmaf(v.w, f, y.w));
+            float4 v[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] = u[x];
+            const float f = exp2_fast(__ldcg(part_ml(b)).x - M);
+            if (b < b1) read(b + 1);
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+              o[4 * x] = fmaf(v[x].x, f, o[4 * x]);
+              o[4 * x + 1] = fmaf(v[x].y, f, o[4 * x + 1]);
+              o[4 * x + 2] = fmaf(v[x].z, f, o[4 * x + 2]);
+              o[4 * x + 3] = fmaf(v[x].w, f, o[4 * x + 3]);
+            }
           }
-          reinterpret_cast<uint4*>(out)[c] = make_uint4(pack2(x.x * inv, x.y * inv, T()), pack2(x.z * inv, x.w * inv, T()),
-                                                        pack2(y.x * inv, y.y * inv, T()), pack2(y.z * inv, y.w * inv, T()));
+          store(c, o, inv);
         }
+        flush();
       }
+      TILE_PIECE_DONE(n);
     }
   } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ------------------------------------------------------------------ pages to operands
-    const int ct = tid - 256, row = ct >> 3, c = ct & 7;        // key row % 16, 16 dims from 16 c on
-    const uint32_t half = (uint32_t)(c >> 2) * kHalf, c16 = (c & 3) * 2;
-    uint32_t it = 0;
-    for (Walk k(batch); k.more(); k.next()) {
-      const Item key(a, k.sp, k.G, k.blk);
-      // lane g < 8 of each warp looks up 16-key group g of a tile
-      auto page_of = [&](int i) {
-        const int j = key.key(i) + 16 * lane;
-        int page = -1;
-        if (lane < kGroups && i < k.t1 && key.seen(j, 16)) {
-          page = page_at(a.b, a.c, k.s, j / ps);
-          if (page < 0) set_status(a.status, UWC_DEV_RANGE);
-        }
-        return page;
-      };
-      auto fetch = [&](const int8_t* data, int page, int j0, uint4* x) {
+    // a thread: key row % 16 and 16 dims from 16 c on; eight lanes of a store have eight rows (no bank conflict)
+    const int wv = warp - 8, row = 8 * (wv & 1) + (lane & 7), c = 4 * (wv >> 1) + (lane >> 3);
+    const uint32_t off = (uint32_t)(wv >> 1) * kHalf + row * 128;
+    const uint32_t off0 = off + (((2 * (lane >> 3)) ^ (row & 7)) << 4), off1 = off + (((2 * (lane >> 3) + 1) ^ (row & 7)) << 4);
+    auto fetch = [&](const int8_t* data, uint32_t t, uint4* x) {
 #pragma unroll
-        for (int g = 0; g < kGroups; g++) {
-          const int pg = __shfl_sync(0xffffffffu, page, g);
-          x[g] = make_uint4(0, 0, 0, 0);
-          if (pg >= 0)
-            x[g] = __ldg(reinterpret_cast<const uint4*>(data + (((size_t)pg * Hkv + k.h) * ps + (j0 + 16 * g) % ps + row) * kHd) + c);
-        }
-      };
-      auto store = [&](uint32_t base, const uint4* x) {
+      for (int g = 0; g < kGroups; g++) {
+        const int y = s_row[t % kPageRing][g];
+        x[g] = make_uint4(0, 0, 0, 0);
+        if (y >= 0) x[g] = __ldg(reinterpret_cast<const uint4*>(data + (size_t)(y + row) * kHd) + c);
+      }
+    };
+    auto store = [&](uint32_t base, const uint4* x) {
 #pragma unroll
-        for (int g = 0; g < kGroups; g++) {
-          const uint32_t u[4] = {x[g].x ^ 0x80808080u, x[g].y ^ 0x80808080u, x[g].z ^ 0x80808080u, x[g].w ^ 0x80808080u};
-          const uint4 lo = make_uint4(i8_half2(u[0], 0x4140), i8_half2(u[0], 0x4342), i8_half2(u[1], 0x4140), i8_half2(u[1], 0x4342));
-          const uint4 hi = make_uint4(i8_half2(u[2], 0x4140), i8_half2(u[2], 0x4342), i8_half2(u[3], 0x4140), i8_half2(u[3], 0x4342));
-          const uint32_t at = base + half + (16 * g + row) * 128;
-          const uint32_t a0 = at + ((c16 ^ (row & 7)) << 4), a1 = at + (((c16 + 1) ^ (row & 7)) << 4);
-          // the two blocks' threads write opposite halves of a row pair at a time: no bank conflict
-          const bool swap = c >= 4;
-          sts128(swap ? a1 : a0, swap ? hi : lo);
-          sts128(swap ? a0 : a1, swap ? lo : hi);
-        }
-      };
-      uint4 x[kGroups], y[kGroups];
-      int page = page_of(k.t0);
-      fetch(a.c.k, page, key.key(k.t0), x);
-      for (int i = k.t0; i < k.t1; i++, it++) {
-        const int st = it & 1;
-        const uint32_t use = it >> 1;
-        const int j0 = key.key(i), npage = i + 1 < k.t1 ? page_of(i + 1) : -1;
-        float2 sc = make_float2(-1.f, 0.f);
-        if (ct < kGroups && page >= 0) {
-          const size_t ph = (size_t)page * Hkv + k.h;
-          sc = make_float2(__ldg(a.c.sk + ph), __ldg(a.c.sv + ph));
-        }
-        fetch(a.c.v, page, j0, y);
-        if (use > 0) TILE_WAIT(bar.k_empty[st], (use - 1) & 1);
+      for (int g = 0; g < kGroups; g++) {
+        const uint32_t u[4] = {x[g].x ^ 0x80808080u, x[g].y ^ 0x80808080u, x[g].z ^ 0x80808080u, x[g].w ^ 0x80808080u};
+        const uint4 lo = make_uint4(i8_half2(u[0], 0x4140), i8_half2(u[0], 0x4342), i8_half2(u[1], 0x4140), i8_half2(u[1], 0x4342));
+        const uint4 hi = make_uint4(i8_half2(u[2], 0x4140), i8_half2(u[2], 0x4342), i8_half2(u[3], 0x4140), i8_half2(u[3], 0x4342));
+        sts128(base + off0 + 16 * g * 128, lo);
+        sts128(base + off1 + 16 * g * 128, hi);
+      }
+    };
+    // the tiles of all pieces are one stream: tile t's loads are issued while tile t - 1 is stored
+    uint4 x[kGroups], y[kGroups];
+#pragma unroll 1
+    for (uint32_t nx = 0;; nx++) {
+      const uint32_t t = nx - 1, st = t & 1;       // stored here; nothing yet when nx = 0
+      TILE_WAIT(bar.page_full[nx % kAhead], (nx / kAhead) & 1);
+      const bool more = s_row[nx % kPageRing][0] != -2;
+      if (nx > 0) {
+        if (t > 1) TILE_WAIT(bar.k_empty[st], ((t >> 1) - 1) & 1);
         store(smK + st * kOperand, x);
-        if (ct < kGroups) s_scale[it % kScaleRing][ct] = sc;
         fence_async_smem();
-        mbar_arrive(&bar.k_full[st]);
-        if (i + 1 < k.t1) fetch(a.c.k, npage, key.key(i + 1), x);
-        if (use > 0) TILE_WAIT(bar.v_empty[st], (use - 1) & 1);
+        warp_arrive(&bar.k_full[st]);
+      }
+      if (more) fetch(a.c.k, nx, x);
+      if (nx > 0) {
+        if (t > 1) TILE_WAIT(bar.v_empty[st], ((t >> 1) - 1) & 1);
         store(smV + st * kOperand, y);
         fence_async_smem();
-        mbar_arrive(&bar.v_full[st]);
-        page = npage;
+        warp_arrive(&bar.v_full[st]);
       }
+      if (!more) break;
+      fetch(a.c.v, nx, y);
+      warp_arrive(&bar.page_empty[nx % kAhead]);
     }
   } else {
-    // ------------------------------------------------------------------ the products
-    uint32_t it = 0, items[2] = {0, 0}, n1 = 0;   // tiles; items of each row tile; tiles of the second row tile
-    for (Walk k(batch); k.more(); k.next()) {
-      const int nw = k.rows(1) > 0 ? 2 : 1;
-      const uint32_t itw[2] = {it, n1};           // each row tile's own count of tiles (its barriers' phases)
-      const int T1 = k.t1 - k.t0;
-      auto scores = [&](int st, int w) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 13) {
+      // ---------------------------------------------------------------- the walk along this CTA's part of the line
+      Start p = s_start;
+      Span sp = batch.span(p.s);
+      int blks = batch.blocks(sp);
+#pragma unroll 1
+      for (uint32_t n = 0;; n++) {
+        const int slot = n % kPieces;
+        if (n >= kPieces) TILE_WAIT(bar.piece_empty[slot], (n / kPieces - 1) & 1);
+        Piece& k = s_piece[slot];
+        int done = 0;
+        if (p.left > 0) {
+          const Item it(a, sp, G, p.blk);
+          const int t1 = min(it.total, p.t0 + p.left);
+          done = t1 - p.t0;
+          if (lane == 0) {
+            k.first = 2 * kRows * p.blk;
+            k.rows = min(2 * kRows, sp.n * G - 2 * kRows * p.blk);
+            k.row0 = sp.row0;
+            k.seq = p.s;
+            k.head = p.h;
+            k.start = sp.idle ? -1 : sp.start;
+            k.t0 = p.t0;
+            k.t1 = t1;
+            k.whole = done == it.total;
+            // the CTAs before this one hold t0 of the item's tiles, those after it the rest, `per` each
+            if (done < it.total) {
+              k.b0 = blockIdx.x - (p.t0 > 0 ? (uint32_t)(p.t0 - 1) / (uint32_t)p.per + 1 : 0);
+              k.b1 = blockIdx.x + (it.total > t1 ? (uint32_t)(it.total - t1 - 1) / (uint32_t)p.per + 1 : 0);
+            }
+            k.lo = it.lo;
+            k.hi = it.hi;
+            k.sink_end = it.sink_end;
+            k.tA = it.tA;
+            k.tB0 = it.tB0;
+          }
+        } else if (lane == 0) {
+          k.rows = 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.piece_full[slot]);
+        if (done == 0) break;
+        p.left -= done;
+        p.t0 = 0;
+        if (p.left > 0 && ++p.blk == blks) {
+          p.blk = 0;
+          if (++p.h == Hkv) {
+            p.h = 0;
+            do {
+              sp = batch.span(++p.s);
+              blks = batch.blocks(sp);
+            } while (blks == 0 && p.s + 1 < a.b.seqs);
+          }
+        }
+      }
+    } else if (warp == 14) {
+      // ---------------------------------------------------------------- the pages: a lane a 16-key group, four tiles at once
+      const int grp = lane & (kGroups - 1);
+      uint32_t t = 0;
+#pragma unroll 1
+      for (uint32_t n = 0;; n++) {
+        TILE_PIECE(n);
+        auto look = [&](int i0, int& y, float2& sc) {
+          const int i = i0 + lane / kGroups, j = k.key(i) + 16 * grp;
+          y = -1;
+          sc = make_float2(-1.f, 0.f);
+          if (i < k.t1 && k.seen(j, 16)) {
+            const int page = page_at(a.b, a.c, k.seq, j >> a.c.lg);
+            if (page < 0) {
+              set_status(a.status, UWC_DEV_RANGE);
+            } else {
+              const int ph = page * Hkv + k.head;      // rows of the pool fit an int: the host checks
+              y = ph * ps + (j & (ps - 1));
+              sc = make_float2(__ldg(a.c.sk + ph), __ldg(a.c.sv + ph));
+            }
+          }
+        };
+        int y = -1, ny;
+        float2 sc = make_float2(-1.f, 0.f), nsc;
+        // the look-up of four tiles ahead of their hand-over
+#pragma unroll 1
+        for (int i0 = k.t0 - kAhead; i0 < k.t1; i0 += kAhead) {
+          look(i0 + kAhead, ny, nsc);
+#pragma unroll 1
+          for (int i = 0; i < kAhead && i0 >= k.t0 && i0 + i < k.t1; i++, t++) {
+            if (t >= kAhead) TILE_WAIT(bar.page_empty[t % kAhead], (t / kAhead - 1) & 1);
+            if (lane / kGroups == i) {
+              s_row[t % kPageRing][grp] = y;
+              s_scale[t % kPageRing][grp] = sc;
+            }
+            warp_arrive(&bar.page_full[t % kAhead]);
+          }
+          y = ny;
+          sc = nsc;
+        }
+        TILE_PIECE_DONE(n);
+      }
+      if (t >= kAhead) TILE_WAIT(bar.page_empty[t % kAhead], (t / kAhead - 1) & 1);
+      if (lane == 0) {
+        s_row[t % kPageRing][0] = -2;
+        mbar_arrive(&bar.page_full[t % kAhead]);
+      }
+    } else if (warp == 12) {
+      // ------------------------------------------------------------------ the products
+      // (nothing here is indexed by the row tile at run time: a local array would wait for the L2 cache)
+      uint32_t it = 0, it0 = 0, it1 = 0, q0 = 0, q1 = 0;   // tiles; tiles and items of each row tile (its barriers' phases)
+      auto scores = [&](uint32_t st, int w) {
 #pragma unroll
         for (int x = 0; x < 8; x++) {
           const uint32_t off = (x >> 2) * kHalf + (x & 3) * 32;
           mma_ss(tmem + w * 128, sdesc_sw128(smQ + w * kOperand + off), sdesc_sw128(smK + st * kOperand + off), kIdescS, x > 0);
         }
+        mbar_arrive(&bar.s_full[w]);
+        mma_commit(&bar.s_full[w]);
       };
-      // the first tile's scores
-      TILE_WAIT(bar.k_full[it & 1], (it >> 1) & 1);
-      for (int w = 0; w < nw; w++) {
-        TILE_WAIT(bar.q_full[w], items[w] & 1);
+      auto outputs = [&](uint32_t st, int w, int part, uint32_t acc) {   // 64 keys
+#pragma unroll
+        for (int x = 4 * part; x < 4 * part + 4; x++)
+          mma_ts(tmem + 256 + w * 128, tmem + w * 128 + 64 * part + (x & 3) * 8, sdesc_mn(smV + st * kOperand + x * 2048), kIdescO, acc || x > 4 * part);
+      };
+#pragma unroll 1
+      for (uint32_t n = 0;; n++) {
+        TILE_PIECE(n);
+        const bool both = k.rows > kRows;
+        const int T1 = k.t1 - k.t0;
+        TILE_PIECE_DONE(n);
+        // the first tile's scores
+        TILE_WAIT(bar.k_full[it & 1], (it >> 1) & 1);
+        TILE_WAIT(bar.q_full[0], q0 & 1);
         tc_fence_after();
         if (elect_one()) {
-          scores(it & 1, w);
-          mbar_arrive(&bar.s_full[w]);
-          mma_commit(&bar.s_full[w]);
-          if (w == nw - 1) mma_commit(&bar.k_empty[it & 1]);
+          scores(it & 1, 0);
+          if (!both) mma_commit(&bar.k_empty[it & 1]);
         }
         __syncwarp();
-      }
-      for (int j = 0; j < T1; j++, it++) {
-        const uint32_t st = it & 1, nx = it + 1;
-        for (int w = 0; w < nw; w++) {
-          if (w == 0) TILE_WAIT(bar.v_full[st], (it >> 1) & 1);
-          TILE_WAIT(bar.p_full[w], (itw[w] + j) & 1);
-          if (w == 0 && j + 1 < T1) TILE_WAIT(bar.k_full[nx & 1], (nx >> 1) & 1);
+        q0++;
+        if (both) {
+          TILE_WAIT(bar.q_full[1], q1 & 1);
           tc_fence_after();
           if (elect_one()) {
-#pragma unroll
-            for (int x = 0; x < 8; x++)
-              mma_ts(tmem + 256 + w * 128, tmem + w * 128 + x * 8, sdesc_mn(smV + st * kOperand + x * 2048), kIdescO, j > 0 || x > 0);
-            mma_commit(&bar.o_done[w]);
-            if (w == nw - 1) mma_commit(&bar.v_empty[st]);
-            if (j + 1 < T1) {
-              scores(nx & 1, w);
-              mbar_arrive(&bar.s_full[w]);
-              mma_commit(&bar.s_full[w]);
-              if (w == nw - 1) mma_commit(&bar.k_empty[nx & 1]);
-            }
+            scores(it & 1, 1);
+            mma_commit(&bar.k_empty[it & 1]);
           }
           __syncwarp();
+          q1++;
         }
-      }
-      items[0]++;
-      if (nw == 2) {
-        items[1]++;
-        n1 += T1;
+#pragma unroll 1
+        for (int j = 0; j < T1; j++, it++, it0++) {
+          const uint32_t st = it & 1, nx = it + 1;
+          const bool more = j + 1 < T1;
+          TILE_WAIT(bar.v_full[st], (it >> 1) & 1);
+          TILE_WAIT(bar.p_full[0][1], it0 & 1);
+          tc_fence_after();
+          if (elect_one()) outputs(st, 0, 1, j > 0);
+          __syncwarp();
+          TILE_WAIT(bar.p_full[0][0], it0 & 1);
+          tc_fence_after();
+          if (elect_one()) {
+            outputs(st, 0, 0, 1);
+            mma_commit(&bar.o_done[0]);
+            if (!both) mma_commit(&bar.v_empty[st]);
+          }
+          __syncwarp();
+          if (more) {
+            TILE_WAIT(bar.k_full[nx & 1], (nx >> 1) & 1);
+            tc_fence_after();
+            if (elect_one()) {
+              scores(nx & 1, 0);
+              if (!both) mma_commit(&bar.k_empty[nx & 1]);
+            }
+            __syncwarp();
+          }
+          if (both) {
+            TILE_WAIT(bar.p_full[1][1], it1 & 1);
+            tc_fence_after();
+            if (elect_one()) outputs(st, 1, 1, j > 0);
+            __syncwarp();
+            TILE_WAIT(bar.p_full[1][0], it1 & 1);
+            tc_fence_after();
+            if (elect_one()) {
+              outputs(st, 1, 0, 1);
+              mma_commit(&bar.o_done[1]);
+              mma_commit(&bar.v_empty[st]);
+              if (more) {
+                scores(nx & 1, 1);
+                mma_commit(&bar.k_empty[nx & 1]);
+              }
+            }
+            __syncwarp();
+            it1++;
+          }
+        }
       }
     }
   }
-done:
+  if (false) {
+  timeout:
+    if (lane == 0) set_status(a.status, UWC_DEV_TIMEOUT);
+  }
   __syncwarp();
   if (warp == 12) {
     // every product that was issued has landed before the tensor memory goes (bounded, as every wait)
     if (elect_one()) mma_commit(&bar.fin);
     __syncwarp();
+#pragma unroll 1
     for (int n = 0; n < (1 << 20) && !mbar_try_wait(&bar.fin, 0); n++) {
     }
   }
