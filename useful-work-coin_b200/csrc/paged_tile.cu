@@ -7,10 +7,9 @@
 // Roles of a CTA (one per SM, 16 warps; registers go from the others to the softmax):
 //   warps 0-3, 4-7   the softmax of the first and second 128 rows, a row a thread: scores from TMEM, the
 //                    running maximum and sum in float32 registers, weights back to TMEM as fp16 over the
-//                    scores that they came from. They also turn the queries to fp16 and write the output.
-//   warps 8-11       pages to operands: 128 keys of int8 from HBM through registers (a tile ahead) to fp16
-//                    in shared memory (the integers are exact; a byte permute and a subtraction a pair), two
-//                    stages each for keys and values. No scale is multiplied in: the key scale multiplies the
+//                    scores that they came from. They also fetch the queries and write the output.
+//   warps 8-11       pages to operands: 128 keys of int8 from HBM through registers (a tile ahead) to 16 bits
+//                    in shared memory (exact: keys in the queries' type, values in fp16), two stages of each. No scale is multiplied in: the key scale multiplies the
 //                    score, the value scale (over a reference that follows its size) the weight.
 //   warp 12          one thread issues the products: while one row tile is in its softmax the other's run.
 //   warp 13          walks the line (below) and hands the pieces to the others.
@@ -211,6 +210,25 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
+// Two of four int8 values in the queries' type, exactly. bf16 has 8 significant bits, so the byte goes in
+// parts: 0x4300 | its low seven bits is 128 + they, and 0x4300 | its top bit is 128, or 256 for a negative one.
+__device__ __forceinline__ uint32_t i8_pair(uint32_t x, uint32_t sel, __half) { return i8_half2(x ^ 0x80808080u, sel); }
+__device__ __forceinline__ uint32_t i8_pair(uint32_t x, uint32_t sel, __nv_bfloat16) {
+  const uint32_t lo = __byte_perm(x & 0x7f7f7f7fu, 0x43434343u, sel), top = __byte_perm(x & 0x80808080u, 0x43434343u, sel);
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&top));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+struct IsBf16 { static constexpr uint32_t value = 0; };
+template <>
+struct IsBf16<__nv_bfloat16> { static constexpr uint32_t value = 1; };
+
+// What the softmax needs of a tile's pages: the largest value scale, and its 16-key groups that nobody sees.
+struct TileInfo {
+  float vmax;
+  int unseen;
+};
+
 struct Bars {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
 };
@@ -268,7 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   uint8_t* sm = reinterpret_cast<uint8_t*>(((uintptr_t)sm_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bar;
   __shared__ Piece s_piece[kPieces];
-  __shared__ __align__(16) float2 s_scale[kPageRing][kGroups];   // key scale (-1: no key of the group is seen), value scale
+  __shared__ __align__(16) float2 s_scale[kPageRing][kGroups];   // factor of scores (log2), value scale
+  __shared__ TileInfo s_tile[kPageRing];
   __shared__ int s_row[kPageRing][kGroups];        // first cache row of the group's keys (-1: none; -2: no more tiles)
   __shared__ Start s_start;
   __shared__ uint32_t s_tmem;
@@ -326,74 +345,48 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
     const float inv_g = 1.0f / (float)G;
     uint32_t it = 0, all = 0, wgp = 0;             // this warpgroup's tiles, every tile, its barrier's phases
 #pragma unroll 1
+    // Row x of an item is token (x + rem) / G past the item's first one: a division of small numbers, exact in
+    // float32 while they are below 2^20.
+    auto token_of = [&](int x) { return (int)(((float)x + 0.5f) * inv_g); };
+    // Sends a piece's query rows on their way to this warp's part of the operand, two rows a step.
+    auto fetch_q = [&](const Piece& k) {
+      const int rows = min(kRows, k.rows - kRows * w);
+      if (rows <= 0) return;
+      const int tok0 = k.first / G, y = kRows * w + r + k.first - tok0 * G, tok = token_of(y), head = y - tok * G, c = lane & 15;
+      const T* q = reinterpret_cast<const T*>(a.q) + (long long)(k.row0 + tok0) * a.q_tok + (long long)(k.head * G) * a.q_head + 8 * c;
+      const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf;
+#pragma unroll 2
+      for (int i = 0; i < 16; i++) {
+        const int x = 2 * i + (lane >> 4), rr = 32 * (warp & 3) + x;
+        const int tk = __shfl_sync(0xffffffffu, tok, x), hd = __shfl_sync(0xffffffffu, head, x);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)),
+                     "l"(rr < rows ? q + tk * a.q_tok + hd * a.q_head : q), "r"(rr < rows ? 16 : 0)
+                     : "memory");
+      }
+    };
+    TILE_WAIT(bar.piece_full[0], 0);
+    fetch_q(s_piece[0]);
+#pragma unroll 1
     for (uint32_t n = 0;; n++) {
       TILE_PIECE(n);
       const int rows = min(kRows, k.rows - kRows * w);
       if (rows <= 0) {                             // only w = 1: the second tile of a short item
         all += k.t1 - k.t0;
+        TILE_WAIT(bar.piece_full[(n + 1) % kPieces], ((n + 1) / kPieces) & 1);
+        fetch_q(s_piece[(n + 1) % kPieces]);
         TILE_PIECE_DONE(n);
         continue;
       }
-      // row x of the item is token tok0 + (x + rem0) / G of the sequence: a division of small numbers, exact in
-      // float32 while they are below 2^20. A lane keeps its own row's (token - tok0, head of the group).
-      const int tok0 = k.first / G, rem0 = k.first - tok0 * G;
-      auto token_of = [&](int x) { return (int)(((float)(x + rem0) + 0.5f) * inv_g); };
-      const int my_tok = token_of(kRows * w + r), my_head = kRows * w + r + rem0 - my_tok * G;
-      const bool live = r < rows;
-      const int pos = live && k.start >= 0 ? k.start + tok0 + my_tok : -1;
-      // ---- the query rows, two a warp at a time, into their places in the swizzled operand, ...
-      {
-        const int c = lane & 15;
-        const T* q = reinterpret_cast<const T*>(a.q) + (long long)(k.row0 + tok0) * a.q_tok + (long long)(k.head * G) * a.q_head + 8 * c;
-        const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf;
-#pragma unroll 2
-        for (int i = 0; i < 16; i++) {
-          const int x = 2 * i + (lane >> 4), rr = 32 * (warp & 3) + x;
-          const int tk = __shfl_sync(0xffffffffu, my_tok, x), hd = __shfl_sync(0xffffffffu, my_head, x);
-          const uint32_t dst = at + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(rr < rows ? q + tk * a.q_tok + hd * a.q_head : q),
-                       "r"(rr < rows ? 16 : 0)
-                       : "memory");
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncwarp();
-      }
-      // ... where each thread turns its own row to fp16, its largest value at 2^14
-      float qmul;
-      {
-        const uint32_t at = smQ + w * kOperand + r * 128;
-        float mx = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {
-          const uint4 x = lds128(at + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4));
-          const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float2 f = two_f(u[j], T());
-            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-        const int e = row_exponent(mx);
-        const float up = a.scale < 0.f ? -pow2i(e) : pow2i(e);   // a negative scale goes with the query
-        qmul = fabsf(a.scale) * kLog2OfE * pow2i(-e);
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {
-          const uint32_t place = at + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4);
-          const uint4 x = lds128(place);
-          uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float2 f = two_f(u[j], T());
-            u[j] = pack2(f.x * up, f.y * up, __half());
-          }
-          sts128(place, make_uint4(u[0], u[1], u[2], u[3]));
-        }
-      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_async_smem();
       warp_arrive(&bar.q_full[w]);
+      const int tok0 = k.first / G, rem0 = k.first - tok0 * G;
+      const int my_tok = token_of(kRows * w + r + rem0), my_head = kRows * w + r + rem0 - my_tok * G;
+      const bool live = r < rows;
+      const int pos = live && k.start >= 0 ? k.start + tok0 + my_tok : -1;
       // positions of this warpgroup's first and last row bound where its masks are needed
-      const int pa = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w);
-      const int pb = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rows - 1);
+      const int pa = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rem0);
+      const int pb = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rows - 1 + rem0);
       float m = kNoMax, l = 0.f, ref = 0.f;
 #pragma unroll 1
       for (int i = k.t0; i < k.t1; i++, it++, all++) {
@@ -403,9 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         const float2* sc = s_scale[all % kPageRing];
         uint32_t s0[32], s1[32];
         auto load = [&](int c, uint32_t* s) { tmem_ld_32x32b_x32(tS + 32 * c, s); };
-        // whether some key is hidden from some row: past its position, out of its window, without a page
-        bool hidden = j0 + kTile - 1 > pa || (a.window >= 0 && !(j0 > pb - a.window || j0 + kTile <= a.sinks));
-        float kf[kGroups], vf[kGroups], vs = 0.f;
+        float kf[kGroups], vf[kGroups];            // the pages' factors for scores (log2) and values
 #pragma unroll
         for (int g = 0; g < kGroups; g += 2) {
           const uint4 x = lds128(smem_u32(sc + g));
@@ -414,12 +405,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           kf[g + 1] = __uint_as_float(x.z);
           vf[g + 1] = __uint_as_float(x.w);
         }
-#pragma unroll
-        for (int g = 0; g < kGroups; g++) {
-          hidden |= kf[g] < 0.f;
-          vs = fmaxf(vs, vf[g]);
-          kf[g] = fmaxf(kf[g] * qmul, 1e-37f);     // a page's factor for scores (log2); not 0: a hidden score stays -inf
-        }
+        const float vs = s_tile[all % kPageRing].vmax;
+        const int unseen = s_tile[all % kPageRing].unseen;
+        // whether some key is hidden from some row: past its position, out of its window, without a page
+        const bool hidden = j0 + kTile - 1 > pa || (a.window >= 0 && !(j0 > pb - a.window || j0 + kTile <= a.sinks)) || unseen;
         if (hidden) {
           // only tiles at an edge: their hidden scores become -inf where they are, in a rolled loop (the code
           // around it is straight-line, and every instruction of it is fetched for every tile)
@@ -428,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             load(c, s0);
             tmem_wait_ld();
             const int last = pos - j0 - 32 * c, from = a.window < 0 ? -kTile : last - a.window, sink = a.sinks - j0 - 32 * c;
-            const bool g0 = sc[2 * c].x < 0.f, g1 = sc[2 * c + 1].x < 0.f;
+            const bool g0 = unseen >> (2 * c) & 1, g1 = unseen >> (2 * c + 1) & 1;
 #pragma unroll
             for (int x = 0; x < 32; x++)
               s0[x] = x > last || (x <= from && x >= sink) || (x < 16 ? g0 : g1) ? 0xff800000u : s0[x];
@@ -523,32 +512,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         }
         l += (lo_of(l2[0]) + hi_of(l2[0])) + (lo_of(l2[1]) + hi_of(l2[1]));
       }
-      // ---- the item's (or the part's) result
+      // ---- the item's (or the part's) result; the next item's queries come meanwhile
+      TILE_WAIT(bar.piece_full[(n + 1) % kPieces], ((n + 1) / kPieces) & 1);
+      fetch_q(s_piece[(n + 1) % kPieces]);
       TILE_WAIT(bar.o_done[w], (it - 1) & 1);
       tc_fence_after();
       const float back = ref * (1.f / kWeightUnit);
-      // through this warp's rows of the (idle) query operand, so that a row of the output leaves in one piece
-      auto store = [&](int c, const float* o, float f) {             // 32 columns
-        const uint32_t at = smQ + w * kOperand + (c >> 1) * kHalf + r * 128;
+      uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((size_t)(k.row0 + tok0 + my_tok) * a.H + k.head * G + my_head) * kHd);
+      auto store = [&](int c, const float* o, float f) {             // 32 columns of this thread's row
+        if (!live) return;
 #pragma unroll
         for (int x = 0; x < 4; x++)
-          sts128(at + (((4 * (c & 1) + x) ^ (r & 7)) << 4),
-                 make_uint4(pack2(o[8 * x] * f, o[8 * x + 1] * f, T()), pack2(o[8 * x + 2] * f, o[8 * x + 3] * f, T()),
-                            pack2(o[8 * x + 4] * f, o[8 * x + 5] * f, T()), pack2(o[8 * x + 6] * f, o[8 * x + 7] * f, T())));
-      };
-      auto flush = [&]() {
-        __syncwarp();
-        const int c = lane & 15;
-        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((size_t)(k.row0 + tok0) * a.H + k.head * G) * kHd) + c;
-        const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf;
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {
-          const int x = 2 * i + (lane >> 4), rr = 32 * (warp & 3) + x;
-          const int row = __shfl_sync(0xffffffffu, my_tok * a.H + my_head, x);   // of the item's first token's
-          const uint4 v = lds128(at + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
-          if (rr < rows) out[(long long)row * (kHd / 8)] = v;
-        }
-        __syncwarp();
+          out[4 * c + x] = make_uint4(pack2(o[8 * x] * f, o[8 * x + 1] * f, T()), pack2(o[8 * x + 2] * f, o[8 * x + 3] * f, T()),
+                                      pack2(o[8 * x + 4] * f, o[8 * x + 5] * f, T()), pack2(o[8 * x + 6] * f, o[8 * x + 7] * f, T()));
       };
       if (k.whole) {
         const float inv = l == 0.f ? 0.f : back / l;
@@ -560,7 +536,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           store(c, reinterpret_cast<const float*>(s), inv);
         }
         tc_fence_before();
-        flush();
         TILE_PIECE_DONE(n);
         continue;
       }
@@ -634,12 +609,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           }
           store(c, o, inv);
         }
-        flush();
       }
       TILE_PIECE_DONE(n);
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ------------------------------------------------------------------ pages to operands
     // a thread: key row % 16 and 16 dims from 16 c on; eight lanes of a store have eight rows (no bank conflict)
     const int wv = warp - 8, row = 8 * (wv & 1) + (lane & 7), c = 4 * (wv >> 1) + (lane >> 3);
@@ -651,6 +625,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         const int y = s_row[t % kPageRing][g];
         x[g] = make_uint4(0, 0, 0, 0);
         if (y >= 0) x[g] = __ldg(reinterpret_cast<const uint4*>(data + (size_t)(y + row) * kHd) + c);
+      }
+    };
+    const uint32_t negate = a.scale < 0.f ? 0x80008000u : 0u;   // a negative scale goes with the keys
+    auto store_k = [&](uint32_t base, const uint4* x) {
+#pragma unroll
+      for (int g = 0; g < kGroups; g++) {
+        const uint32_t u[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          v[2 * i] = i8_pair(u[i], 0x4140, T());
+          v[2 * i + 1] = i8_pair(u[i], 0x4342, T());
+        }
+        if (negate)
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] ^= negate;
+        sts128(base + off0 + 16 * g * 128, make_uint4(v[0], v[1], v[2], v[3]));
+        sts128(base + off1 + 16 * g * 128, make_uint4(v[4], v[5], v[6], v[7]));
       }
     };
     auto store = [&](uint32_t base, const uint4* x) {
@@ -672,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       const bool more = s_row[nx % kPageRing][0] != -2;
       if (nx > 0) {
         if (t > 1) TILE_WAIT(bar.k_empty[st], ((t >> 1) - 1) & 1);
-        store(smK + st * kOperand, x);
+        store_k(smK + st * kOperand, x);
         fence_async_smem();
         warp_arrive(&bar.k_full[st]);
       }
@@ -688,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       warp_arrive(&bar.page_empty[nx % kAhead]);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 13) {
       // ---------------------------------------------------------------- the walk along this CTA's part of the line
       Start p = s_start;
@@ -747,6 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
     } else if (warp == 14) {
       // ---------------------------------------------------------------- the pages: a lane a 16-key group, four tiles at once
       const int grp = lane & (kGroups - 1);
+      const float qmul = fabsf(a.scale) * kLog2OfE;
       uint32_t t = 0;
 #pragma unroll 1
       for (uint32_t n = 0;; n++) {
@@ -754,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         auto look = [&](int i0, int& y, float2& sc) {
           const int i = i0 + lane / kGroups, j = k.key(i) + 16 * grp;
           y = -1;
-          sc = make_float2(-1.f, 0.f);
+          sc = make_float2(1e-37f, 0.f);
           if (i < k.t1 && k.seen(j, 16)) {
             const int page = page_at(a.b, a.c, k.seq, j >> a.c.lg);
             if (page < 0) {
@@ -762,12 +755,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             } else {
               const int ph = page * Hkv + k.head;      // rows of the pool fit an int: the host checks
               y = ph * ps + (j & (ps - 1));
-              sc = make_float2(__ldg(a.c.sk + ph), __ldg(a.c.sv + ph));
+              // the factor of scores is not 0, so that a hidden score stays -inf
+              sc = make_float2(fmaxf(__ldg(a.c.sk + ph) * qmul, 1e-37f), __ldg(a.c.sv + ph));
             }
           }
         };
         int y = -1, ny;
-        float2 sc = make_float2(-1.f, 0.f), nsc;
+        float2 sc = make_float2(1e-37f, 0.f), nsc;
         // the look-up of four tiles ahead of their hand-over
 #pragma unroll 1
         for (int i0 = k.t0 - kAhead; i0 < k.t1; i0 += kAhead) {
@@ -775,9 +769,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
 #pragma unroll 1
           for (int i = 0; i < kAhead && i0 >= k.t0 && i0 + i < k.t1; i++, t++) {
             if (t >= kAhead) TILE_WAIT(bar.page_empty[t % kAhead], (t / kAhead - 1) & 1);
+            float vmax = sc.y;
+#pragma unroll
+            for (int o = 1; o < kGroups; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+            const unsigned unseen = __ballot_sync(0xffffffffu, y < 0) >> (i * kGroups) & ((1u << kGroups) - 1);
             if (lane / kGroups == i) {
               s_row[t % kPageRing][grp] = y;
               s_scale[t % kPageRing][grp] = sc;
+              if (grp == 0) s_tile[t % kPageRing] = TileInfo{vmax, (int)unseen};
             }
             warp_arrive(&bar.page_full[t % kAhead]);
           }
@@ -799,7 +798,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
 #pragma unroll
         for (int x = 0; x < 8; x++) {
           const uint32_t off = (x >> 2) * kHalf + (x & 3) * 32;
-          mma_ss(tmem + w * 128, sdesc_sw128(smQ + w * kOperand + off), sdesc_sw128(smK + st * kOperand + off), kIdescS, x > 0);
+          mma_ss(tmem + w * 128, sdesc_sw128(smQ + w * kOperand + off), sdesc_sw128(smK + st * kOperand + off),
+                 kIdescS | IsBf16<T>::value * ((1u << 7) | (1u << 10)), x > 0);
         }
         mbar_arrive(&bar.s_full[w]);
         mma_commit(&bar.s_full[w]);
