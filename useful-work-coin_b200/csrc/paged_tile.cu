@@ -40,8 +40,9 @@ constexpr int kPageRing = 8;                 // slots: those, and up to four tha
 constexpr int kSeqs = 1024;                  // sequences whose span and tiles are kept in shared memory
 constexpr int kSmem = 1024 + 6 * kOperand + kSeqs * 24;   // two query tiles, two stages of keys, two of values
 constexpr int kMinTiles = 4;                 // a CTA's least share of the line
-constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-constexpr uint32_t kIdescO = kIdescS | (1u << 16);   // values are stored key by key: B is MN-major
+constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+// 128 dims; values are stored key by key: B is MN-major
+constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(kHd >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 constexpr float kRaise = 4.f;                // log2 by which a score may pass the running maximum
 constexpr float kWeightUnit = 1024.f;         // the fp16 weight of p = 1 at the reference scale
 
@@ -230,7 +231,7 @@ struct TileInfo {
 };
 
 struct Bars {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
 };
 
 // Pairs of float32 (one instruction for two), and the larger of three.
@@ -301,7 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       mbar_init(&bar.k_empty[i], 1);
       mbar_init(&bar.v_full[i], 4);
       mbar_init(&bar.v_empty[i], 1);
-      mbar_init(&bar.s_full[i], 2);
+      mbar_init(&bar.s_full[i][0], 2);
+      mbar_init(&bar.s_full[i][1], 2);
       mbar_init(&bar.p_full[i][0], 4);
       mbar_init(&bar.p_full[i][1], 4);
       mbar_init(&bar.o_done[i], 1);
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   const int Hkv = a.c.Hkv, ps = a.c.ps, G = a.H / Hkv;
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     // ------------------------------------------------------------------ softmax, a row a thread
     const int w = warp >> 2, r = tid & (kRows - 1);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -388,42 +390,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       const int pa = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rem0);
       const int pb = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rows - 1 + rem0);
       float m = kNoMax, l = 0.f, ref = 0.f;
+      // 64 keys a step; the next step's scores are being computed meanwhile, in the other half of this row
+      // tile's score columns
 #pragma unroll 1
-      for (int i = k.t0; i < k.t1; i++, it++, all++) {
-        const int j0 = k.key(i);
-        TILE_WAIT(bar.s_full[w], it & 1);
+      for (int u = 2 * k.t0; u < 2 * k.t1; u++, it++) {
+        const int h = u & 1, j0 = k.key(u >> 1) + 64 * h;
+        const uint32_t tH = tS + 64 * h, slot = all % kPageRing;
+        all += h;
+        TILE_WAIT(bar.s_full[w][h], (it >> 1) & 1);
         tc_fence_after();
-        const float2* sc = s_scale[all % kPageRing];
         uint32_t s0[32], s1[32];
-        auto load = [&](int c, uint32_t* s) { tmem_ld_32x32b_x32(tS + 32 * c, s); };
-        float kf[kGroups], vf[kGroups];            // the pages' factors for scores (log2) and values
+        tmem_ld_32x32b_x32(tH, s0);
+        float kf[4], vf[4];                        // the pages' factors for scores (log2) and values
 #pragma unroll
-        for (int g = 0; g < kGroups; g += 2) {
-          const uint4 x = lds128(smem_u32(sc + g));
+        for (int g = 0; g < 4; g += 2) {
+          const uint4 x = lds128(smem_u32(&s_scale[slot][4 * h + g]));
           kf[g] = __uint_as_float(x.x);
           vf[g] = __uint_as_float(x.y);
           kf[g + 1] = __uint_as_float(x.z);
           vf[g + 1] = __uint_as_float(x.w);
         }
-        const float vs = s_tile[all % kPageRing].vmax;
-        const int unseen = s_tile[all % kPageRing].unseen;
+        const float vs = s_tile[slot].vmax;
+        const int unseen = s_tile[slot].unseen >> (4 * h) & 15;
         // whether some key is hidden from some row: past its position, out of its window, without a page
-        const bool hidden = j0 + kTile - 1 > pa || (a.window >= 0 && !(j0 > pb - a.window || j0 + kTile <= a.sinks)) || unseen;
+        const bool hidden = j0 + 63 > pa || (a.window >= 0 && !(j0 > pb - a.window || j0 + 64 <= a.sinks)) || unseen;
         if (hidden) {
-          // only tiles at an edge: their hidden scores become -inf where they are, in a rolled loop (the code
-          // around it is straight-line, and every instruction of it is fetched for every tile)
+          // only keys at an edge: their hidden scores become -inf where they are, in a rolled loop (every
+          // instruction of the code around it is fetched for every step)
 #pragma unroll 1
-          for (int c = 0; c < 4; c++) {
-            load(c, s0);
+          for (int c = 0; c < 2; c++) {
+            tmem_ld_32x32b_x32(tH + 32 * c, s0);
             tmem_wait_ld();
             const int last = pos - j0 - 32 * c, from = a.window < 0 ? -kTile : last - a.window, sink = a.sinks - j0 - 32 * c;
             const bool g0 = unseen >> (2 * c) & 1, g1 = unseen >> (2 * c + 1) & 1;
 #pragma unroll
             for (int x = 0; x < 32; x++)
               s0[x] = x > last || (x <= from && x >= sink) || (x < 16 ? g0 : g1) ? 0xff800000u : s0[x];
-            tmem_st_32x32b_x32(tS + 32 * c, s0);
+            tmem_st_32x32b_x32(tH + 32 * c, s0);
           }
           tmem_wait_st();
+          tmem_ld_32x32b_x32(tH, s0);
         }
         float mx = kNoMax;
         auto top = [&](const uint32_t* s, float f0, float f1) {
@@ -439,18 +445,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             mx = fmaxf(mx, fmaxf(u, v) * (g ? f1 : f0));
           }
         };
-        // 32 columns at a time, the next ones on their way. Rolled: the straight-line form needs 11 KB of
-        // instructions for every tile, and waits for them
-        load(0, s0);
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          tmem_wait_ld();
-          load(c + 1, s1);
-          top(s0, c ? kf[4] : kf[0], c ? kf[5] : kf[1]);
-          tmem_wait_ld();
-          load(2, s0);
-          top(s1, c ? kf[6] : kf[2], c ? kf[7] : kf[3]);
-        }
+        tmem_wait_ld();
+        tmem_ld_32x32b_x32(tH + 32, s1);
+        top(s0, kf[0], kf[1]);
+        tmem_wait_ld();
+        top(s1, kf[2], kf[3]);
         // ---- raise the maximum or the value reference, and bring O along (its products must be done)
         const bool raise = mx > m + kRaise, refer = vs > 2.f * ref || (vs > 0.f && vs < ref * (1.f / 64.f));
         if (__any_sync(0xffffffffu, raise || refer)) {
@@ -460,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           l *= down;
           m = m2;
           ref = ref2;
-          if (i > k.t0) {
+          if (u > 2 * k.t0) {
             TILE_WAIT(bar.o_done[w], (it - 1) & 1);
             tc_fence_after();
 #pragma unroll 1
@@ -474,8 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             }
           }
         }
-        // ---- weights: p = 2^(score - m); the row sum keeps p, the product gets p s_v / ref in fp16. The
-        // last 64 keys' product starts while the others' weights are computed.
+        // ---- weights: p = 2^(score - m); the row sum keeps p, the product gets p s_v / ref in fp16, over the
+        // scores that they came from
         const float unit = ref > 0.f ? __fdividef(kWeightUnit, ref) : 0.f;
         const uint64_t nm = two(-m, -m);
         uint64_t l2[2] = {0ull, 0ull};
@@ -496,20 +495,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             }
           }
         };
-        // keys 64 .. 127 first, over their own scores, then keys 0 .. 63
-#pragma unroll 1
-        for (int h = 1; h >= 0; h--) {
-          tmem_wait_ld();
-          load(2 * h + 1, s1);
-          weigh(s0, p, h ? kf[4] : kf[0], h ? kf[5] : kf[1], h ? vf[4] : vf[0], h ? vf[5] : vf[1]);
-          tmem_wait_ld();
-          if (h) load(0, s0);
-          weigh(s1, p + 16, h ? kf[6] : kf[2], h ? kf[7] : kf[3], h ? vf[6] : vf[2], h ? vf[7] : vf[3]);
-          tmem_st_32x32b_x32(tS + 64 * h, p);
-          tmem_wait_st();
-          tc_fence_before();
-          warp_arrive(&bar.p_full[w][h]);
-        }
+        weigh(s0, p, kf[0], kf[1], vf[0], vf[1]);
+        weigh(s1, p + 16, kf[2], kf[3], vf[2], vf[3]);
+        tmem_st_32x32b_x32(tH, p);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(&bar.p_full[w][h]);
         l += (lo_of(l2[0]) + hi_of(l2[0])) + (lo_of(l2[1]) + hi_of(l2[1]));
       }
       // ---- the item's (or the part's) result; the next item's queries come meanwhile
@@ -680,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       warp_arrive(&bar.page_empty[nx % kAhead]);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     if (warp == 13) {
       // ---------------------------------------------------------------- the walk along this CTA's part of the line
       Start p = s_start;
@@ -794,20 +785,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       // ------------------------------------------------------------------ the products
       // (nothing here is indexed by the row tile at run time: a local array would wait for the L2 cache)
       uint32_t it = 0, it0 = 0, it1 = 0, q0 = 0, q1 = 0;   // tiles; tiles and items of each row tile (its barriers' phases)
-      auto scores = [&](uint32_t st, int w) {
+      auto scores = [&](uint32_t st, int w, uint32_t h) {  // 64 keys
+        const uint32_t d = tmem + w * 128 + 64 * h, q = smQ + w * kOperand, kk = smK + st * kOperand + h * 64 * 128;
 #pragma unroll
         for (int x = 0; x < 8; x++) {
           const uint32_t off = (x >> 2) * kHalf + (x & 3) * 32;
-          mma_ss(tmem + w * 128, sdesc_sw128(smQ + w * kOperand + off), sdesc_sw128(smK + st * kOperand + off),
-                 kIdescS | IsBf16<T>::value * ((1u << 7) | (1u << 10)), x > 0);
+          mma_ss(d, sdesc_sw128(q + off), sdesc_sw128(kk + off), kIdescS | IsBf16<T>::value * ((1u << 7) | (1u << 10)), x > 0);
         }
-        mbar_arrive(&bar.s_full[w]);
-        mma_commit(&bar.s_full[w]);
+        mbar_arrive(&bar.s_full[w][h]);
+        mma_commit(&bar.s_full[w][h]);
       };
-      auto outputs = [&](uint32_t st, int w, int part, uint32_t acc) {   // 64 keys
+      auto outputs = [&](uint32_t st, int w, uint32_t h, uint32_t acc) {
+        const uint32_t p = tmem + w * 128 + 64 * h, v = smV + st * kOperand + h * 8192;
 #pragma unroll
-        for (int x = 4 * part; x < 4 * part + 4; x++)
-          mma_ts(tmem + 256 + w * 128, tmem + w * 128 + 64 * part + (x & 3) * 8, sdesc_mn(smV + st * kOperand + x * 2048), kIdescO, acc || x > 4 * part);
+        for (int x = 0; x < 4; x++) mma_ts(tmem + 256 + w * 128, p + 8 * x, sdesc_mn(v + x * 2048), kIdescO, acc || x > 0);
+        mma_commit(&bar.o_done[w]);
       };
 #pragma unroll 1
       for (uint32_t n = 0;; n++) {
@@ -818,68 +810,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         // the first tile's scores
         TILE_WAIT(bar.k_full[it & 1], (it >> 1) & 1);
         TILE_WAIT(bar.q_full[0], q0 & 1);
+        if (both) TILE_WAIT(bar.q_full[1], q1 & 1);
         tc_fence_after();
         if (elect_one()) {
-          scores(it & 1, 0);
-          if (!both) mma_commit(&bar.k_empty[it & 1]);
+#pragma unroll 1
+          for (uint32_t h = 0; h < 2; h++) {
+            scores(it & 1, 0, h);
+            if (both) scores(it & 1, 1, h);
+          }
+          mma_commit(&bar.k_empty[it & 1]);
         }
         __syncwarp();
         q0++;
-        if (both) {
-          TILE_WAIT(bar.q_full[1], q1 & 1);
-          tc_fence_after();
-          if (elect_one()) {
-            scores(it & 1, 1);
-            mma_commit(&bar.k_empty[it & 1]);
-          }
-          __syncwarp();
-          q1++;
-        }
+        q1 += both;
 #pragma unroll 1
-        for (int j = 0; j < T1; j++, it++, it0++) {
+        for (int j = 0; j < T1; j++, it++, it0++, it1 += both) {
           const uint32_t st = it & 1, nx = it + 1;
           const bool more = j + 1 < T1;
           TILE_WAIT(bar.v_full[st], (it >> 1) & 1);
-          TILE_WAIT(bar.p_full[0][1], it0 & 1);
-          tc_fence_after();
-          if (elect_one()) outputs(st, 0, 1, j > 0);
-          __syncwarp();
-          TILE_WAIT(bar.p_full[0][0], it0 & 1);
-          tc_fence_after();
-          if (elect_one()) {
-            outputs(st, 0, 0, 1);
-            mma_commit(&bar.o_done[0]);
-            if (!both) mma_commit(&bar.v_empty[st]);
-          }
-          __syncwarp();
-          if (more) {
-            TILE_WAIT(bar.k_full[nx & 1], (nx >> 1) & 1);
+          if (more) TILE_WAIT(bar.k_full[nx & 1], (nx >> 1) & 1);
+#pragma unroll 1
+          for (uint32_t h = 0; h < 2; h++) {
+            TILE_WAIT(bar.p_full[0][h], it0 & 1);
             tc_fence_after();
             if (elect_one()) {
-              scores(nx & 1, 0);
-              if (!both) mma_commit(&bar.k_empty[nx & 1]);
+              outputs(st, 0, h, j > 0 || h > 0);
+              if (more) scores(nx & 1, 0, h);
             }
             __syncwarp();
-          }
-          if (both) {
-            TILE_WAIT(bar.p_full[1][1], it1 & 1);
-            tc_fence_after();
-            if (elect_one()) outputs(st, 1, 1, j > 0);
-            __syncwarp();
-            TILE_WAIT(bar.p_full[1][0], it1 & 1);
-            tc_fence_after();
-            if (elect_one()) {
-              outputs(st, 1, 0, 1);
-              mma_commit(&bar.o_done[1]);
-              mma_commit(&bar.v_empty[st]);
-              if (more) {
-                scores(nx & 1, 1);
-                mma_commit(&bar.k_empty[nx & 1]);
+            if (both) {
+              TILE_WAIT(bar.p_full[1][h], it1 & 1);
+              tc_fence_after();
+              if (elect_one()) {
+                outputs(st, 1, h, j > 0 || h > 0);
+                if (more) scores(nx & 1, 1, h);
               }
+              __syncwarp();
             }
-            __syncwarp();
-            it1++;
           }
+          if (elect_one()) {
+            mma_commit(&bar.v_empty[st]);
+            if (more) mma_commit(&bar.k_empty[nx & 1]);
+          }
+          __syncwarp();
         }
       }
     }
