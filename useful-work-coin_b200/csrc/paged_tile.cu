@@ -231,7 +231,7 @@ struct TileInfo {
 };
 
 struct Bars {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
 };
 
 // Pairs of float32 (one instruction for two), and the larger of three.
@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       mbar_init(&bar.s_full[i][1], 2);
       mbar_init(&bar.p_full[i][0], 4);
       mbar_init(&bar.p_full[i][1], 4);
-      mbar_init(&bar.o_done[i], 1);
+      mbar_init(&bar.o_done[i][0], 1);
+      mbar_init(&bar.o_done[i][1], 1);
       mbar_init(&bar.wg[i], 4);
     }
     mbar_init(&bar.fin, 1);
@@ -460,7 +461,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           m = m2;
           ref = ref2;
           if (u > 2 * k.t0) {
-            TILE_WAIT(bar.o_done[w], (it - 1) & 1);
+            // the step before's (that these scores are there says that those before it are done, so this
+            // barrier is at most one phase behind: a wait cannot tell more)
+            TILE_WAIT(bar.o_done[w][h ^ 1], ((it - 1) >> 1) & 1);
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < 8; c++) {
@@ -506,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       // ---- the item's (or the part's) result; the next item's queries come meanwhile
       TILE_WAIT(bar.piece_full[(n + 1) % kPieces], ((n + 1) / kPieces) & 1);
       fetch_q(s_piece[(n + 1) % kPieces]);
-      TILE_WAIT(bar.o_done[w], (it - 1) & 1);
+      TILE_WAIT(bar.o_done[w][0], ((it - 1) >> 1) & 1);
+      TILE_WAIT(bar.o_done[w][1], ((it - 1) >> 1) & 1);
       tc_fence_after();
       const float back = ref * (1.f / kWeightUnit);
       uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((size_t)(k.row0 + tok0 + my_tok) * a.H + k.head * G + my_head) * kHd);
@@ -799,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         const uint32_t p = tmem + w * 128 + 64 * h, v = smV + st * kOperand + h * 8192;
 #pragma unroll
         for (int x = 0; x < 4; x++) mma_ts(tmem + 256 + w * 128, p + 8 * x, sdesc_mn(v + x * 2048), kIdescO, acc || x > 0);
-        mma_commit(&bar.o_done[w]);
+        mma_commit(&bar.o_done[w][h]);
       };
 #pragma unroll 1
       for (uint32_t n = 0;; n++) {
