@@ -478,8 +478,8 @@ int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t* vc, const 
  * H a multiple of Hkv (head h reads KV head h / (H / Hkv)); out (rows, H, 128) contiguous, in dtype.
  * softmax(scale q . k) in float32; a row that sees no key is zero. No atomics touch a result: the same
  * call gives the same bits. workspace: uwc_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
- * zero before its first use; every call leaves its counters zero again. Calls that overlap on the GPU
- * must not share one. */
+ * whose first 4096 are zero before its first use (counters; every call leaves them zero). Calls that
+ * overlap on the GPU must not share one. */
 uint64_t uwc_paged_attention_workspace_bytes(int seqs, int max_new, int max_len, int H, int Hkv, int window,
                                              int sinks);
 int uwc_paged_attention(const int8_t* kc, const float* sk, const int8_t* vc, const float* sv, int pages, int page_size,

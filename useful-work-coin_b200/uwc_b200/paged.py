@@ -25,6 +25,7 @@ from ._lib import check, lib
 HD = 128
 PAGE_SIZES = (16, 32, 64, 128)
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_SCALE = 1.0 / math.sqrt(HD)
 
 
 def new_cache(pages: int, Hkv: int, page_size: int = 64, device="cuda") -> dict:
@@ -36,34 +37,38 @@ def new_cache(pages: int, Hkv: int, page_size: int = 64, device="cuda") -> dict:
                 sk=z(pages, Hkv, dt=torch.float32), sv=z(pages, Hkv, dt=torch.float32))
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
+I8, I32, F32, BF16, F16 = torch.int8, torch.int32, torch.float32, torch.bfloat16, torch.float16
+
+
 def _cache_args(cache: dict, table, start, cu):
-    """The cache's and the batch's pointers and sizes, checked."""
+    """The cache's and the batch's pointers and sizes, checked, and their device."""
     k, v, sk, sv = cache["k"], cache["v"], cache["sk"], cache["sv"]
-    pages, Hkv, ps, hd = k.shape
-    assert hd == HD and v.shape == k.shape and sk.shape == (pages, Hkv) and sv.shape == (pages, Hkv), (k.shape, sk.shape)
-    assert k.dtype == torch.int8 and v.dtype == torch.int8 and sk.dtype == torch.float32 and sv.dtype == torch.float32
-    assert k.is_cuda and k.is_contiguous() and v.is_contiguous() and sk.is_contiguous() and sv.is_contiguous()
-    assert table.dtype == torch.int32 and start.dtype == torch.int32 and cu.dtype == torch.int32
+    shape = pages, Hkv, ps, hd = k.shape
+    scales = (pages, Hkv)
+    assert hd == HD and v.shape == shape and sk.shape == scales and sv.shape == scales, (shape, sk.shape, sv.shape)
+    assert k.dtype is I8 and v.dtype is I8 and sk.dtype is F32 and sv.dtype is F32
+    assert table.dtype is I32 and start.dtype is I32 and cu.dtype is I32
     seqs, width = table.shape
     assert start.shape == (seqs,) and cu.shape == (seqs + 1,), (table.shape, start.shape, cu.shape)
-    assert table.is_contiguous() and start.is_contiguous() and cu.is_contiguous()
-    dev = k.device
-    for t in (v, sk, sv, table, start, cu):
-        assert t.device == dev, "the cache and the batch's description lie on one device"
+    assert (k.is_contiguous() and v.is_contiguous() and sk.is_contiguous() and sv.is_contiguous()
+            and table.is_contiguous() and start.is_contiguous() and cu.is_contiguous())
+    dev = k.get_device()
+    assert (dev >= 0 and v.get_device() == dev and sk.get_device() == dev and sv.get_device() == dev
+            and table.get_device() == dev and start.get_device() == dev and cu.get_device() == dev), \
+        "the cache and the batch's description lie on one CUDA device"
+    assert dev == _device(), "the tensors' device is the current one"
     return (k.data_ptr(), sk.data_ptr(), v.data_ptr(), sv.data_ptr(), pages, ps, Hkv, table.data_ptr(),
             start.data_ptr(), cu.data_ptr(), seqs, width), dev
 
 
-def _rows(t: torch.Tensor, n: int, heads: int, dtype, dev):
+def _rows(t: torch.Tensor, n: int, heads: int, dtype, dev: int):
     """(pointer, token stride, head stride) of a row tensor (n, heads, 128)."""
-    assert t.shape == (n, heads, HD) and t.dtype == dtype and t.device == dev, (t.shape, t.dtype, t.device)
-    assert t.stride(2) == 1, "a head's 128 values are contiguous"
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
-def _current(dev) -> int:
-    assert dev.index == torch.cuda.current_device(), "the tensors' device is the current one"
-    return torch.cuda.current_stream(dev).cuda_stream
+    assert t.shape == (n, heads, HD) and t.dtype is dtype and t.get_device() == dev, (t.shape, t.dtype, t.device)
+    tok, head, one = t.stride()
+    assert one == 1, "a head's 128 values are contiguous"
+    return t.data_ptr(), tok, head
 
 
 def append(k, v, cache: dict, table, start, cu, max_new: int, cos, sin, q=None, q_norm=None, k_norm=None,
@@ -77,21 +82,24 @@ def append(k, v, cache: dict, table, start, cu, max_new: int, cos, sin, q=None, 
     already there are brought to it. Appending the same tokens again changes nothing."""
     args, dev = _cache_args(cache, table, start, cu)
     n, Hkv, dt = k.shape[0], args[6], k.dtype
-    assert dt in (torch.bfloat16, torch.float16), dt
+    assert dt is BF16 or dt is F16, dt
     kr, vr = _rows(k, n, Hkv, dt, dev), _rows(v, n, Hkv, dt, dev)
-    assert cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.shape == sin.shape and cos.shape[1] == HD
-    assert cos.is_contiguous() and sin.is_contiguous() and cos.device == dev and sin.device == dev
-    for w in (q_norm, k_norm):
-        assert w is None or (w.shape == (HD,) and w.dtype == torch.float32 and w.is_contiguous() and w.device == dev)
-    out, H, qr = None, 0, (None, 0, 0)
+    max_pos, hd = cos.shape
+    assert hd == HD and sin.shape == cos.shape and cos.dtype is F32 and sin.dtype is F32, (cos.shape, sin.shape)
+    assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == dev and sin.get_device() == dev
+    qn = kn = None
+    if q_norm is not None or k_norm is not None:
+        for w in (q_norm, k_norm):
+            assert w is None or (w.shape == (HD,) and w.dtype is F32 and w.is_contiguous() and w.get_device() == dev)
+        qn, kn = (None if w is None else w.data_ptr() for w in (q_norm, k_norm))
+    out, po, H, qr = None, None, 0, (None, 0, 0)
     if q is not None:
         H = q.shape[1]
         qr = _rows(q, n, H, dt, dev)
-        out = torch.empty((n, H, HD), dtype=dt, device=dev)
-    ptr = lambda t: None if t is None else t.data_ptr()
-    check(lib().uwc_paged_append(*args, n, max_new, _TYPES[dt], *kr, *vr, *qr, ptr(out), H, cos.data_ptr(),
-                                 sin.data_ptr(), cos.shape[0], ptr(q_norm), ptr(k_norm), eps, _current(dev)),
-          "paged append")
+        out = torch.empty((n, H, HD), dtype=dt, device=q.device)
+        po = out.data_ptr()
+    check(lib().uwc_paged_append(*args, n, max_new, 0 if dt is BF16 else 1, *kr, *vr, *qr, po, H, cos.data_ptr(),
+                                 sin.data_ptr(), max_pos, qn, kn, eps, _raw_stream(dev)), "paged append")
     return out
 
 
@@ -99,26 +107,33 @@ def gather(cache: dict, table, first, cu, n: int, max_rows: int, dtype=torch.bfl
     """Cached tokens as values: rows cu[s] .. cu[s + 1] - 1 of the two (n, Hkv, 128) tensors returned
     are sequence s's keys and values at positions first[s] and on (at most max_rows of a sequence)."""
     args, dev = _cache_args(cache, table, first, cu)
-    k = torch.empty((n, args[6], HD), dtype=dtype, device=dev)
+    k = torch.empty((n, args[6], HD), dtype=dtype, device=table.device)
     v = torch.empty_like(k)
-    check(lib().uwc_paged_gather(*args, n, max_rows, _TYPES[dtype], k.data_ptr(), v.data_ptr(), _current(dev)),
+    check(lib().uwc_paged_gather(*args, n, max_rows, _TYPES[dtype], k.data_ptr(), v.data_ptr(), _raw_stream(dev)),
           "paged gather")
     return k, v
 
 
-_WS: dict = {}       # (device, stream) -> workspace, grown on demand
-_RETIRED: list = []  # outgrown workspaces: a captured graph may still run on one
+_WS: dict = {}       # (device, stream) -> its calls' workspace
+_COUNTERS = 4096     # bytes at a workspace's start that are zero before a call, and after it
 
 
-def _workspace(dev, stream: int, nbytes: int):
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)     # the graph's own, zeroed by it
-    ws = _WS.get((dev.index, stream))
-    if ws is None or ws.numel() < nbytes:
+def _workspace(device, dev: int, stream: int, shape):
+    """The stream's workspace, as large as any call needs (40 MB), its counters zeroed once: a call leaves
+    them so. A captured call gets one of its own size, whose counters the graph zeroes."""
+    if not torch.cuda.is_current_stream_capturing():
+        ws = _WS.get((dev, stream))
         if ws is not None:
-            _RETIRED.append(ws)
-            nbytes = max(nbytes, 2 * ws.numel())
-        ws = _WS[(dev.index, stream)] = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+            return ws
+        big = 1 << 30
+        need = lib().uwc_paged_attention_workspace_bytes
+        nbytes = max(need(1, rows, big, 1, 1, -1, 0) for rows in (8, 16, big))
+    else:
+        nbytes = lib().uwc_paged_attention_workspace_bytes(*shape)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws[:_COUNTERS].zero_()
+    if not torch.cuda.is_current_stream_capturing():
+        _WS[(dev, stream)] = ws
     return ws
 
 
@@ -131,21 +146,18 @@ def attention(q, cache: dict, table, start, cu, max_new: int, max_len: int, scal
     args, dev = _cache_args(cache, table, start, cu)
     n, H, _ = q.shape
     dt = q.dtype
-    assert dt in (torch.bfloat16, torch.float16), dt
+    assert dt is BF16 or dt is F16, dt
     assert window is None or window >= 0, window
-    assert 0 <= sinks, sinks
+    assert sinks >= 0, sinks
     qr = _rows(q, n, H, dt, dev)
     if out is None:
-        out = torch.empty((n, H, HD), dtype=dt, device=dev)
-    assert out.shape == (n, H, HD) and out.dtype == dt and out.is_contiguous() and out.device == dev
-    w = -1 if window is None else min(int(window), 1 << 30)
-    sinks = min(int(sinks), 1 << 30)
-    stream = _current(dev)
-    L = lib()
-    nbytes = L.uwc_paged_attention_workspace_bytes(args[10], max_new, max_len, H, args[6], w, sinks)
-    ws = _workspace(dev, stream, nbytes) if nbytes else None
-    check(L.uwc_paged_attention(*args, n, max_new, max_len, _TYPES[dt], *qr, out.data_ptr(), H,
-                                1.0 / math.sqrt(HD) if scale is None else scale, w, sinks,
-                                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream),
+        out = torch.empty((n, H, HD), dtype=dt, device=q.device)
+    else:
+        assert out.shape == (n, H, HD) and out.dtype is dt and out.is_contiguous() and out.get_device() == dev
+    stream = _raw_stream(dev)
+    w, sinks = -1 if window is None else min(window, 1 << 30), min(sinks, 1 << 30)
+    ws = _workspace(q.device, dev, stream, (args[10], max_new, max_len, H, args[6], w, sinks))
+    check(lib().uwc_paged_attention(*args, n, max_new, max_len, 0 if dt is BF16 else 1, *qr, out.data_ptr(), H,
+                                    _SCALE if scale is None else scale, w, sinks, ws.data_ptr(), ws.numel(), stream),
           "paged attention")
     return out
