@@ -27,36 +27,22 @@ using paged::Span;
 using paged::span_of;
 
 constexpr int kThreads = 256;
-constexpr int kQHeads = 4;       // query heads that share a thread's rotation values
+constexpr int kQHeads = 2;       // query heads that share a thread's rotation values
 
-// Eight 16-bit values as float32.
-__device__ __forceinline__ void unpack8(const uint4 w, float* f, __nv_bfloat16) {
+// Eight 16-bit values as float32, and back.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 w, float* f) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    f[2 * i] = __uint_as_float(u[i] << 16);
-    f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    const float2 x = paged::two_f(u[i], T());
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
   }
-}
-__device__ __forceinline__ void unpack8(const uint4 w, float* f, __half) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
-  }
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float* f) {
+  using paged::pack2;
   return make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
 }
 
@@ -77,16 +63,19 @@ struct AppendArgs {
   uint32_t* status;
 };
 
-// A token head lies in eight threads: thread c of them holds dims 8 c .. 8 c + 7 (lo) and their
-// rotation partners 64 + 8 c .. (hi).
+// A token head lies in eight lanes: lane c of them holds dims 8 c .. 8 c + 7 (lo) and their rotation
+// partners 64 + 8 c .. (hi).
+struct Raw {
+  uint4 lo, hi;
+};
 template <typename T>
-__device__ __forceinline__ void load_head(const Rows& r, long long row, int h, int c, float* lo, float* hi) {
+__device__ __forceinline__ Raw load_raw(const Rows& r, long long row, int h, int c) {
   const T* p = reinterpret_cast<const T*>(r.p) + row * r.tok + h * r.head + 8 * c;
-  unpack8(*reinterpret_cast<const uint4*>(p), lo, T());
-  unpack8(*reinterpret_cast<const uint4*>(p + 64), hi, T());
+  return Raw{*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 64)};
 }
 
-// det_rmsnorm over the head (exact fixed-point sum of 128 squares, runtime/detrt/core.py:151-159)
+// det_rmsnorm over the head (exact fixed-point sum of 128 squares, runtime/detrt/core.py:151-159); all
+// lanes of a warp together
 __device__ __forceinline__ void norm_head(const float* __restrict__ w, float eps, int c, float* lo, float* hi) {
   float mx = 0.f;
 #pragma unroll
@@ -112,29 +101,24 @@ __device__ __forceinline__ void norm_head(const float* __restrict__ w, float eps
   }
 }
 
-struct Turn {              // one token's rotation values for a thread's dims
-  float4 v[8];             // cos lo, cos hi, sin lo, sin hi (two float4 each)
+// The rotation values of four dims of a lane (half 0: its first four) and of their partners, and the
+// rotation of those: rows `pos` of the tables.
+struct Turn4 {
+  float4 cl, ch, sl, sh;
 };
-__device__ __forceinline__ Turn load_turn(const float* cos, const float* sin, int pos, int c) {
-  Turn t;
-  const float4* a = reinterpret_cast<const float4*>(cos + (size_t)pos * kHd) + 2 * c;
-  const float4* b = reinterpret_cast<const float4*>(sin + (size_t)pos * kHd) + 2 * c;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    t.v[i] = __ldg(a + i);
-    t.v[2 + i] = __ldg(a + 16 + i);
-    t.v[4 + i] = __ldg(b + i);
-    t.v[6 + i] = __ldg(b + 16 + i);
-  }
-  return t;
+__device__ __forceinline__ Turn4 load_turn(const float* cos, const float* sin, int pos, int c, int half) {
+  const float4* a = reinterpret_cast<const float4*>(cos + (size_t)pos * kHd) + 2 * c + half;
+  const float4* b = reinterpret_cast<const float4*>(sin + (size_t)pos * kHd) + 2 * c + half;
+  return Turn4{__ldg(a), __ldg(a + 16), __ldg(b), __ldg(b + 16)};
 }
-__device__ __forceinline__ void rotate(const Turn& t, float* lo, float* hi) {
-  const float* f = reinterpret_cast<const float*>(t.v);
+__device__ __forceinline__ void rotate4(const Turn4& t, float* lo, float* hi) {
+  const float cl[4] = {t.cl.x, t.cl.y, t.cl.z, t.cl.w}, ch[4] = {t.ch.x, t.ch.y, t.ch.z, t.ch.w};
+  const float sl[4] = {t.sl.x, t.sl.y, t.sl.z, t.sl.w}, sh[4] = {t.sh.x, t.sh.y, t.sh.z, t.sh.w};
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
+  for (int i = 0; i < 4; i++) {
     const float x = lo[i], y = hi[i];
-    lo[i] = __fadd_rn(__fmul_rn(x, f[i]), __fmul_rn(-y, f[16 + i]));
-    hi[i] = __fadd_rn(__fmul_rn(y, f[8 + i]), __fmul_rn(x, f[24 + i]));
+    lo[i] = __fadd_rn(__fmul_rn(x, cl[i]), __fmul_rn(-y, sl[i]));
+    hi[i] = __fadd_rn(__fmul_rn(y, ch[i]), __fmul_rn(x, sh[i]));
   }
 }
 
@@ -143,7 +127,9 @@ __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= FLT_MAX ? a : 0.f;
 }
-__device__ __forceinline__ uint32_t quant4(const float* x, float s) {
+// Four values as clamp(rint(fdiv(x, s)), +-127), NaN as 0.
+__device__ __forceinline__ uint32_t quant4_exact(float4 x4, float s) {
+  const float x[4] = {x4.x, x4.y, x4.z, x4.w};
   uint32_t o = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -153,121 +139,262 @@ __device__ __forceinline__ uint32_t quant4(const float* x, float s) {
   }
   return o;
 }
+// The same without the divisions (half of the kernel's instructions) where that cannot change a bit: inv is
+// 1 / s, so x inv is within 1e-4 of the quotient (|quotient| <= 127), and both round to the same integer
+// unless it lies that near to a half. 1.5 2^23 + x inv has the integer in its low byte. Infinities, NaN and
+// an infinite inv fail the test too.
+__device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t t[4];
+  bool sure = true;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float y = x[i] * inv, z = y + kMagic;
+    t[i] = __float_as_uint(z);
+    sure = sure && fabsf(y - (z - kMagic)) < 0.4999f;
+  }
+  if (!sure) return quant4_exact(make_float4(x[0], x[1], x[2], x[3]), s);
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ float inverse(float s) { return s > 1e-30f ? __frcp_rn(s) : __int_as_float(0x7f800000); }
 
-// Page units: one CTA for the new tokens of one (sequence, touched page, KV head) and of keys or
-// values. The page's new rows stay in registers between their maximum and their quantization (NP
-// passes of 32 token rows). Query units: 32 (token, four query heads) a CTA.
-template <typename T, int NP>
-__global__ void __launch_bounds__(kThreads) k_paged_append(const AppendArgs a) {
+// One row of queries: unit u is (row, four query heads) of eight lanes, four units a warp.
+template <typename T, bool NORM>
+__device__ __forceinline__ void query_unit(const AppendArgs& a, long long u, int c) {
+  const int groups = (a.H + kQHeads - 1) / kQHeads;
+  const int row = (int)(u / groups), h0 = (int)(u % groups) * kQHeads;
+  const bool in = row < a.b.rows;
+  int pos = -1;
+  bool covered = false;
+  Raw raw[kQHeads];
+#pragma unroll
+  for (int i = 0; i < kQHeads; i++) {
+    raw[i] = Raw{};
+    if (in && h0 + i < a.H && !(NORM && a.q_norm)) raw[i] = load_raw<T>(a.q, row, h0 + i, c);
+  }
+  if (in) {
+    // the sequence whose span holds this row: the last with cu[s] <= row
+    int s = 0;
+    for (int n = a.b.seqs; n > 1;) {
+      const int half = n >> 1;
+      if (__ldg(a.b.cu + s + half) <= row) s += half;
+      n -= half;
+    }
+    const Span sp = span_of(a.b, a.c.ps, s);
+    const int t = row - sp.row0;
+    covered = t >= 0 && t < sp.n;
+    if (covered && !sp.idle) {
+      pos = sp.start + t;
+      if (pos >= a.max_pos) {
+        set_status(a.status, UWC_DEV_RANGE);
+        pos = -1;
+      }
+    }
+  }
+  T* out = reinterpret_cast<T*>(a.q_out) + ((size_t)row * a.H + h0) * kHd + 8 * c;
+  if (NORM && a.q_norm) {
+#pragma unroll 1
+    for (int i = 0; i < kQHeads; i++) {
+      float lo[8], hi[8];
+      Raw x = {};
+      if (in && h0 + i < a.H) x = load_raw<T>(a.q, row, h0 + i, c);
+      unpack8<T>(x.lo, lo);
+      unpack8<T>(x.hi, hi);
+      norm_head(a.q_norm, a.eps, c, lo, hi);
+      if (pos >= 0)
+#pragma unroll
+        for (int k = 0; k < 2; k++) rotate4(load_turn(a.cos, a.sin, pos, c, k), lo + 4 * k, hi + 4 * k);
+      if (covered && h0 + i < a.H) {
+        *reinterpret_cast<uint4*>(out + i * kHd) = pos >= 0 ? pack8<T>(lo) : make_uint4(0, 0, 0, 0);   // an idle slot's rows are zero
+        *reinterpret_cast<uint4*>(out + i * kHd + 64) = pos >= 0 ? pack8<T>(hi) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+  // in place, four dims of all four heads at a time: the rotation values are read once
+  if (pos >= 0) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const Turn4 t = load_turn(a.cos, a.sin, pos, c, k);
+#pragma unroll
+      for (int i = 0; i < kQHeads; i++) {
+        uint32_t* lw = reinterpret_cast<uint32_t*>(&raw[i].lo) + 2 * k;
+        uint32_t* hw = reinterpret_cast<uint32_t*>(&raw[i].hi) + 2 * k;
+        const float2 l0 = paged::two_f(lw[0], T()), l1 = paged::two_f(lw[1], T());
+        const float2 h0_ = paged::two_f(hw[0], T()), h1 = paged::two_f(hw[1], T());
+        float lo[4] = {l0.x, l0.y, l1.x, l1.y}, hi[4] = {h0_.x, h0_.y, h1.x, h1.y};
+        rotate4(t, lo, hi);
+        lw[0] = paged::pack2(lo[0], lo[1], T());
+        lw[1] = paged::pack2(lo[2], lo[3], T());
+        hw[0] = paged::pack2(hi[0], hi[1], T());
+        hw[1] = paged::pack2(hi[2], hi[3], T());
+      }
+    }
+  }
+  if (covered)
+#pragma unroll
+    for (int i = 0; i < kQHeads; i++)
+      if (h0 + i < a.H) {
+        *reinterpret_cast<uint4*>(out + i * kHd) = pos >= 0 ? raw[i].lo : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(out + i * kHd + 64) = pos >= 0 ? raw[i].hi : make_uint4(0, 0, 0, 0);
+      }
+}
+
+// A page's part in a call: unit (sequence, touched page, KV head, keys or values).
+struct PageUnit {
+  int p0, p1, base, row0, h;   // positions p0 .. p1 - 1 are written; row of position p: row0 + p
+  bool is_k;
+  int8_t* data;                // the page's (page_size, 128) of the head
+  float* scale;
+};
+__device__ __forceinline__ bool page_unit(const AppendArgs& a, long long unit, bool leader, PageUnit& u) {
+  u.is_k = (unit & 1) == 0;
+  u.h = (int)((unit >> 1) % a.c.Hkv);
+  const int sj = (int)((unit >> 1) / a.c.Hkv), s = sj / a.most, j = sj - s * a.most;
+  const Span sp = span_of(a.b, a.c.ps, s);
+  if (sp.bad && j == 0 && leader) set_status(a.status, UWC_DEV_RANGE);
+  if (sp.idle || sp.n <= 0) return false;
+  const int ps = a.c.ps, slot = (sp.start >> a.c.lg) + j;
+  u.base = slot * ps;
+  u.p0 = max(sp.start, u.base);
+  u.p1 = min(sp.start + sp.n, u.base + ps);        // positions written here
+  if (u.p0 >= u.p1) return false;
+  u.row0 = sp.row0 - sp.start;
+  const int page = page_at(a.b, a.c, s, slot);
+  if (page < 0 || (u.is_k && u.p1 > a.max_pos)) {
+    if (leader) set_status(a.status, UWC_DEV_RANGE);
+    return false;
+  }
+  const size_t ph = (size_t)page * a.c.Hkv + u.h;
+  u.scale = (u.is_k ? a.c.sk : a.c.sv) + ph;
+  u.data = (u.is_k ? a.c.k : a.c.v) + ph * ps * kHd;
+  return true;
+}
+
+// A lane's 16 values of the row at position p, rotated where they are a key's.
+template <typename T, bool NORM>
+__device__ __forceinline__ void row_values(const AppendArgs& a, const PageUnit& u, const Raw& raw, int p, bool live, int c,
+                                           float* lo, float* hi) {
+  unpack8<T>(raw.lo, lo);
+  unpack8<T>(raw.hi, hi);
+  if (!u.is_k) return;
+  if (NORM && a.k_norm) norm_head(a.k_norm, a.eps, c, lo, hi);
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < 2; i++) rotate4(load_turn(a.cos, a.sin, p, c, i), lo + 4 * i, hi + 4 * i);
+}
+__device__ __forceinline__ float row_max(const float* lo, const float* hi) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = fmaxf(m, fmaxf(finite_abs(lo[i]), finite_abs(hi[i])));
+  return m;
+}
+__device__ __forceinline__ void store_row(const PageUnit& u, int p, int c, const float* lo, const float* hi, float s, float inv) {
+  int8_t* d = u.data + (size_t)(p - u.base) * kHd + 8 * c;
+  *reinterpret_cast<uint2*>(d) = make_uint2(quant4(lo, s, inv), quant4(lo + 4, s, inv));
+  *reinterpret_cast<uint2*>(d + 64) = make_uint2(quant4(hi, s, inv), quant4(hi + 4, s, inv));
+}
+// The tokens that the page already holds, brought from scale s0 to a grown one: n threads, 16 values a step.
+__device__ __forceinline__ void requantize(const PageUnit& u, float s0, float s, float inv, int tid, int n) {
+  uint4* d = reinterpret_cast<uint4*>(u.data);
+#pragma unroll 4
+  for (int w = tid; w < (u.p0 - u.base) * (kHd / 16); w += n) {
+    const uint4 x = d[w];
+    uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) f[i] = __fmul_rn((float)(int8_t)(y[k] >> (8 * i)), s0);
+      y[k] = quant4(f, s, inv);
+    }
+    d[w] = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+}
+
+// Prompts: one CTA a page unit, its rows in NP passes of 32. All rows' loads are issued first and stay
+// packed (16 bits); without a norm a key is rotated twice, for the maximum and for its quantization, which
+// costs less than the registers that would hold it: at 64 registers instead of 86 the SM has four CTAs'
+// loads in flight, not two (8 x 2048 tokens of 16 + 2 x 8 heads: 66 us, 121 us before).
+template <typename T, int NP, bool NORM>
+__global__ void __launch_bounds__(kThreads, NORM ? 2 : NP == 4 ? 3 : 4) k_paged_append(const AppendArgs a) {
   const int tid = threadIdx.x, c = tid & 7, r8 = tid >> 3;
   const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
   if (blockIdx.x >= units) {
-    // ---- queries
-    const int groups = (a.H + kQHeads - 1) / kQHeads;
-    const long long u = (blockIdx.x - units) * (kThreads / 8) + r8;
-    const int row = (int)(u / groups), h0 = (int)(u % groups) * kQHeads;
-    const bool in = row < a.b.rows;
-    int pos = -1;
-    bool covered = false;
-    if (in) {
-      // the sequence whose span holds this row: the last with cu[s] <= row
-      int s = 0;
-      for (int n = a.b.seqs; n > 1;) {
-        const int half = n >> 1;
-        if (__ldg(a.b.cu + s + half) <= row) s += half;
-        n -= half;
-      }
-      const Span sp = span_of(a.b, a.c.ps, s);
-      const int t = row - sp.row0;
-      covered = t >= 0 && t < sp.n;
-      if (covered && !sp.idle) {
-        pos = sp.start + t;
-        if (pos >= a.max_pos) {
-          set_status(a.status, UWC_DEV_RANGE);
-          pos = -1;
-        }
-      }
-    }
-    // (all threads stay for the norm's shuffles)
-    Turn tn = {};
-    if (pos >= 0) tn = load_turn(a.cos, a.sin, pos, c);
-#pragma unroll
-    for (int i = 0; i < kQHeads; i++) {
-      const int h = h0 + i;
-      float lo[8] = {}, hi[8] = {};
-      if (pos >= 0 && h < a.H) load_head<T>(a.q, row, h, c, lo, hi);
-      if (a.q_norm) norm_head(a.q_norm, a.eps, c, lo, hi);
-      if (pos >= 0) rotate(tn, lo, hi);
-      else
-#pragma unroll
-        for (int j = 0; j < 8; j++) lo[j] = hi[j] = 0.f;
-      if (covered && h < a.H) {
-        T* o = reinterpret_cast<T*>(a.q_out) + ((size_t)row * a.H + h) * kHd + 8 * c;
-        *reinterpret_cast<uint4*>(o) = pack8<T>(lo);
-        *reinterpret_cast<uint4*>(o + 64) = pack8<T>(hi);
-      }
-    }
+    query_unit<T, NORM>(a, (blockIdx.x - units) * (kThreads / 8) + r8, c);
     return;
   }
-  // ---- keys and values
-  const int unit = blockIdx.x;
-  const bool is_k = (unit & 1) == 0;
-  const int h = (unit >> 1) % a.c.Hkv, sj = (unit >> 1) / a.c.Hkv;
-  const int s = sj / a.most, j = sj % a.most;
-  const Span sp = span_of(a.b, a.c.ps, s);
-  if (sp.bad && j == 0 && tid == 0) set_status(a.status, UWC_DEV_RANGE);
-  if (sp.idle || sp.n <= 0) return;
-  const int ps = a.c.ps, slot = (sp.start >> a.c.lg) + j, base = slot * ps;
-  const int p0 = max(sp.start, base), p1 = min(sp.start + sp.n, base + ps);   // positions written here
-  if (p0 >= p1) return;
-  const int page = page_at(a.b, a.c, s, slot);
-  if (page < 0 || (is_k && p1 > a.max_pos)) {
-    if (tid == 0) set_status(a.status, UWC_DEV_RANGE);
-    return;
-  }
-  const size_t ph = (size_t)page * a.c.Hkv + h;
-  float* scale = (is_k ? a.c.sk : a.c.sv) + ph;
-  int8_t* data = (is_k ? a.c.k : a.c.v) + ph * ps * kHd;
-  const float s0 = p0 > base ? *scale : 0.f;
-  float lo[NP][8], hi[NP][8], amax = 0.f;
+  PageUnit u;
+  if (!page_unit(a, blockIdx.x, tid == 0, u)) return;
+  const float s0 = u.p0 > u.base ? *u.scale : 0.f;
+  Raw raw[NP];
 #pragma unroll
   for (int n = 0; n < NP; n++) {
-    const int p = base + n * 32 + r8;
-    const bool live = p >= p0 && p < p1;
+    const int p = u.base + n * 32 + r8;
+    raw[n] = Raw{};
+    if (p >= u.p0 && p < u.p1) raw[n] = load_raw<T>(u.is_k ? a.k : a.v, u.row0 + p, u.h, c);
+  }
+  float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) lo[n][i] = hi[n][i] = 0.f;
-    if (live) load_head<T>(is_k ? a.k : a.v, sp.row0 + (p - sp.start), h, c, lo[n], hi[n]);
-    if (is_k) {
-      if (a.k_norm) norm_head(a.k_norm, a.eps, c, lo[n], hi[n]);
-      if (live) rotate(load_turn(a.cos, a.sin, p, c), lo[n], hi[n]);
-    }
-    if (live)
-#pragma unroll
-      for (int i = 0; i < 8; i++) amax = fmaxf(amax, fmaxf(finite_abs(lo[n][i]), finite_abs(hi[n][i])));
+  for (int n = 0; n < NP; n++) {
+    const int p = u.base + n * 32 + r8;
+    const bool live = p >= u.p0 && p < u.p1;
+    float lo[8], hi[8];
+    row_values<T, NORM>(a, u, raw[n], p, live, c, lo, hi);
+    if (live) amax = fmaxf(amax, row_max(lo, hi));
   }
   __shared__ float red[kThreads / 32];
   amax = block_maxf<kThreads>(amax, red);
-  const float sn = fmaxf(s0, __fdiv_rn(amax, 127.0f));
+  const float sn = fmaxf(s0, __fdiv_rn(amax, 127.0f)), inv = inverse(sn);
 #pragma unroll
   for (int n = 0; n < NP; n++) {
-    const int p = base + n * 32 + r8;
-    if (p < p0 || p >= p1) continue;
-    int8_t* d = data + (size_t)(p - base) * kHd + 8 * c;
-    *reinterpret_cast<uint2*>(d) = make_uint2(quant4(lo[n], sn), quant4(lo[n] + 4, sn));
-    *reinterpret_cast<uint2*>(d + 64) = make_uint2(quant4(hi[n], sn), quant4(hi[n] + 4, sn));
+    const int p = u.base + n * 32 + r8;
+    const bool live = p >= u.p0 && p < u.p1;
+    float lo[8], hi[8];
+    row_values<T, NORM>(a, u, raw[n], p, live, c, lo, hi);
+    if (live) store_row(u, p, c, lo, hi, sn, inv);
   }
-  if (p0 > base && sn > s0) {
-    // the tokens that the page already holds, brought to the grown scale
-    for (int w = tid; w < (p0 - base) * (kHd / 4); w += kThreads) {
-      uint32_t* d = reinterpret_cast<uint32_t*>(data) + w;
-      const uint32_t x = *d;
-      float f[4];
+  if (u.p0 > u.base && sn > s0) requantize(u, s0, sn, inv, tid, kThreads);
+  if (tid == 0) *u.scale = sn;   // after block_maxf's barriers: every thread has read s0
+}
+
+// Decode steps (at most kFewNew new tokens a sequence): one warp a page unit, so that a batch's units are
+// all resident at once and none waits at a barrier.
+constexpr int kFewNew = 8;
+constexpr int kFewThreads = 128;
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(kFewThreads) k_paged_append_few(const AppendArgs a) {
+  const int lane = threadIdx.x & 31, c = lane & 7, r4 = lane >> 3;
+  const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
+  const long long unit = (long long)blockIdx.x * (kFewThreads / 32) + threadIdx.x / 32;
+  if (unit >= units) {
+    if (a.q.p) query_unit<T, NORM>(a, (unit - units) * 4 + r4, c);
+    return;
+  }
+  PageUnit u;
+  if (!page_unit(a, unit, lane == 0, u)) return;
+  const float s0 = u.p0 > u.base ? *u.scale : 0.f;
+  constexpr int NP = kFewNew / 4;
+  float lo[NP][8], hi[NP][8], amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) f[i] = __fmul_rn((float)(int8_t)(x >> (8 * i)), s0);
-      *d = quant4(f, sn);
-    }
+  for (int n = 0; n < NP; n++) {
+    const int p = u.p0 + 4 * n + r4;
+    const bool live = p < u.p1;
+    Raw raw = {};
+    if (live) raw = load_raw<T>(u.is_k ? a.k : a.v, u.row0 + p, u.h, c);
+    row_values<T, NORM>(a, u, raw, p, live, c, lo[n], hi[n]);
+    if (live) amax = fmaxf(amax, row_max(lo[n], hi[n]));
   }
-  if (tid == 0) *scale = sn;   // after block_maxf's barriers: every thread has read s0
+  amax = warp_maxf(amax);
+  const float sn = fmaxf(s0, __fdiv_rn(amax, 127.0f)), inv = inverse(sn);
+#pragma unroll
+  for (int n = 0; n < NP; n++) {
+    const int p = u.p0 + 4 * n + r4;
+    if (p < u.p1) store_row(u, p, c, lo[n], hi[n], sn, inv);
+  }
+  if (u.p0 > u.base && sn > s0) requantize(u, s0, sn, inv, lane, 32);
+  __syncwarp();
+  if (lane == 0) *u.scale = sn;
 }
 
 struct GatherArgs {
@@ -284,35 +411,34 @@ __device__ __forceinline__ void store8(float* o, const float* f) {
   reinterpret_cast<float4*>(o)[1] = make_float4(f[4], f[5], f[6], f[7]);
 }
 
-// Eight threads a (token, KV head), 16 dims each; 32 of them a CTA, keys and values both.
+// 16 lanes a (token, KV head), eight dims each, keys and values both.
 template <typename O>
 __global__ void __launch_bounds__(kThreads) k_paged_gather(const GatherArgs a) {
   const int s = blockIdx.y;
   const Span sp = span_of(a.b, a.c.ps, s);
   if (sp.bad && blockIdx.x == 0 && threadIdx.x == 0) set_status(a.status, UWC_DEV_RANGE);
-  const long long u = (long long)blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3);
-  const int t = (int)(u / a.c.Hkv), h = (int)(u % a.c.Hkv), c = threadIdx.x & 7;
+  const long long u = (long long)blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
+  const int t = (int)(u / a.c.Hkv), h = (int)(u - (long long)t * a.c.Hkv), c = threadIdx.x & 15;
   if (t >= sp.n) return;
   const int pos = sp.start + t, ps = a.c.ps;
   const int page = sp.idle ? -1 : page_at(a.b, a.c, s, pos >> a.c.lg);
   if (page < 0 && !sp.idle) set_status(a.status, UWC_DEV_RANGE);
-  const size_t out = ((size_t)(sp.row0 + t) * a.c.Hkv + h) * kHd + 16 * c;
+  const size_t out = ((size_t)(sp.row0 + t) * a.c.Hkv + h) * kHd + 8 * c;
+  uint2 w[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+  float sc[2] = {0.f, 0.f};
+  if (page >= 0) {
+    const size_t ph = (size_t)page * a.c.Hkv + h, at = (ph * ps + (pos & (ps - 1))) * kHd + 8 * c;
+    w[0] = *reinterpret_cast<const uint2*>(a.c.k + at);
+    w[1] = *reinterpret_cast<const uint2*>(a.c.v + at);
+    sc[0] = a.c.sk[ph];
+    sc[1] = a.c.sv[ph];
+  }
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    uint4 w = make_uint4(0, 0, 0, 0);
-    float sc = 0.f;
-    if (page >= 0) {
-      const size_t ph = (size_t)page * a.c.Hkv + h;
-      w = *reinterpret_cast<const uint4*>((i ? a.c.v : a.c.k) + (ph * ps + (pos & (ps - 1))) * kHd + 16 * c);
-      sc = (i ? a.c.sv : a.c.sk)[ph];
-    }
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-    float f[16];
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < 16; e++) f[e] = __fmul_rn((float)(int8_t)(x[e >> 2] >> (8 * (e & 3))), sc);
-    O* o = reinterpret_cast<O*>(i ? a.v : a.k) + out;
-    store8(o, f);
-    store8(o + 8, f + 8);
+    for (int e = 0; e < 8; e++) f[e] = __fmul_rn((float)(int8_t)((e < 4 ? w[i].x : w[i].y) >> (8 * (e & 3))), sc[i]);
+    store8(reinterpret_cast<O*>(i ? a.v : a.k) + out, f);
   }
 }
 
@@ -338,13 +464,18 @@ namespace {
 
 bool row_strides_ok(long long tok, long long head) { return tok >= 0 && head >= 0 && tok % 8 == 0 && head % 8 == 0; }
 
-template <typename T>
-int launch_append(const AppendArgs& a, long long grid, cudaStream_t st) {
-  switch (a.c.ps) {
-    case 128: k_paged_append<T, 4><<<(unsigned)grid, kThreads, 0, st>>>(a); break;
-    case 64: k_paged_append<T, 2><<<(unsigned)grid, kThreads, 0, st>>>(a); break;
-    default: k_paged_append<T, 1><<<(unsigned)grid, kThreads, 0, st>>>(a); break;
-  }
+template <typename T, bool NORM>
+int launch_append(const AppendArgs& a, cudaStream_t st) {
+  const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
+  const long long queries = a.q.p ? (long long)a.b.rows * ((a.H + kQHeads - 1) / kQHeads) : 0;
+  const bool few = a.b.max_new <= kFewNew;
+  const long long per = kFewThreads / 32;
+  const long long grid = few ? (units + (queries + 3) / 4 + per - 1) / per : units + (queries * 8 + kThreads - 1) / kThreads;
+  if (grid > 0x7fffffffll) return UWC_ERR_SHAPE;
+  if (few) k_paged_append_few<T, NORM><<<(unsigned)grid, kFewThreads, 0, st>>>(a);
+  else if (a.c.ps == 128) k_paged_append<T, 4, NORM><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  else if (a.c.ps == 64) k_paged_append<T, 2, NORM><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  else k_paged_append<T, 1, NORM><<<(unsigned)grid, kThreads, 0, st>>>(a);
   uwc_count_launch();
   return uwc_launch_status();
 }
@@ -383,11 +514,10 @@ extern "C" int uwc_paged_append(int8_t* kc, float* sk, int8_t* vc, float* sv, in
   a.k_norm = k_norm;
   a.eps = (float)eps;
   a.status = uwc_status_ptr();
-  long long grid = (long long)seqs * a.most * Hkv * 2;
-  if (q) grid += ((long long)rows * ((H + kQHeads - 1) / kQHeads) * 8 + kThreads - 1) / kThreads;
-  if (grid > 0x7fffffffll) return UWC_ERR_SHAPE;
   const cudaStream_t st = (cudaStream_t)stream;
-  return dtype == UWC_T_BF16 ? launch_append<__nv_bfloat16>(a, grid, st) : launch_append<__half>(a, grid, st);
+  const bool norm = q_norm || k_norm;
+  if (dtype == UWC_T_BF16) return norm ? launch_append<__nv_bfloat16, true>(a, st) : launch_append<__nv_bfloat16, false>(a, st);
+  return norm ? launch_append<__half, true>(a, st) : launch_append<__half, false>(a, st);
 }
 
 extern "C" int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t* vc, const float* sv, int pages,
@@ -403,7 +533,7 @@ extern "C" int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t*
   if (!aligned16(k) || !aligned16(v)) return UWC_ERR_ALIGN;
   UWC_CHECK_DEVICE();
   if (seqs == 0 || rows == 0 || max_rows == 0) return UWC_OK;
-  const long long per = ((long long)max_rows * Hkv * 8 + kThreads - 1) / kThreads;
+  const long long per = ((long long)max_rows * Hkv * 16 + kThreads - 1) / kThreads;
   if (per > 0x7fffffffll) return UWC_ERR_SHAPE;
   a.k = k;
   a.v = v;
