@@ -3,7 +3,8 @@
     python useful-work-coin_b200/build.py [--force] [--verbose]
 
 Output: useful-work-coin_b200/uwc_b200/libuwcb200.so, linked against the static CUDA runtime so
-it loads on a machine without a GPU driver (the symbol-export test runs on CPU-only hosts).
+it loads on a machine without a GPU driver (the symbol-export test runs on CPU-only hosts), and beside
+it _paged.so, the torch side of uwc_b200.paged (C++, no device code), linked to it and to torch.
 Nothing is compiled at import time: the product path refuses to run without this library.
 """
 from __future__ import annotations
@@ -29,6 +30,34 @@ def nvcc() -> str:
     return cand if os.path.exists(cand) else "nvcc"
 
 
+EXT_SOURCE = "paged_torch.cpp"
+EXT_OUT = os.path.join(HERE, "uwc_b200", "_paged.so")
+
+
+def build_extension(force: bool = False, verbose: bool = False) -> str:
+    """The torch extension module: calls of the library from tensors."""
+    src = os.path.join(CSRC, EXT_SOURCE)
+    inputs = [src, os.path.join(ROOT, "include", "uwc_b200.h")]
+    if not force and os.path.exists(EXT_OUT) and all(os.path.getmtime(f) <= os.path.getmtime(EXT_OUT) for f in inputs):
+        return EXT_OUT
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = EXT_OUT + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-isystem{d}" for d in includes], src, "-o", tmp, f"-L{libdir}", f"-Wl,-rpath,{libdir}", "-Wl,-rpath,$ORIGIN",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", OUT]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    os.replace(tmp, EXT_OUT)
+    return EXT_OUT
+
+
 def _inputs():
     files = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
     files.append(os.path.join(ROOT, "include", "uwc_b200.h"))
@@ -44,6 +73,7 @@ def up_to_date() -> bool:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
+        build_extension(force, verbose)
         return OUT
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
@@ -58,8 +88,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         objs.append(obj)
     tmp = OUT + ".tmp"
     subprocess.check_call([nvcc(), "-shared", "-cudart", "static", "-gencode", "arch=compute_100a,code=sm_100a",
-                           *objs, "-o", tmp])
+                           "-Xlinker", "-soname=libuwcb200.so", *objs, "-o", tmp])
     os.replace(tmp, OUT)
+    build_extension(force, verbose)
     return OUT
 
 
