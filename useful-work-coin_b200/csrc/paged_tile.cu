@@ -610,10 +610,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ------------------------------------------------------------------ pages to operands
-    // a thread: key row % 16 and 16 dims from 16 c on; eight lanes of a store have eight rows (no bank conflict)
-    const int wv = warp - 8, row = 8 * (wv & 1) + (lane & 7), c = 4 * (wv >> 1) + (lane >> 3);
-    const uint32_t off = (uint32_t)(wv >> 1) * kHalf + row * 128;
-    const uint32_t off0 = off + (((2 * (lane >> 3)) ^ (row & 7)) << 4), off1 = off + (((2 * (lane >> 3) + 1) ^ (row & 7)) << 4);
+    // A thread: key row % 16 and 16 dims from 16 c on. Eight lanes have the eight c of two neighbouring rows, four
+    // of each: neither their loads (a bank each) nor, swizzled into the two blocks, their stores conflict.
+    const int c = lane & 7, row = (4 * (warp - 8) + (lane >> 3)) ^ (c >> 2);
+    const uint32_t off = (uint32_t)(c >> 2) * kHalf + row * 128;
+    const uint32_t off0 = off + (((2 * (c & 3)) ^ (row & 7)) << 4), off1 = off + (((2 * (c & 3) + 1) ^ (row & 7)) << 4);
     auto fetch = [&](const int8_t* data, uint32_t t, uint4* x) {
 #pragma unroll
       for (int g = 0; g < kGroups; g++) {
