@@ -48,7 +48,8 @@ def test_append_refuses(arg, value, code):
 
 @pytest.mark.parametrize("arg,value,code", SHARED + [
     ("start", None, "ARG"), ("q", None, "ARG"), ("out", None, "ARG"), ("dtype", 2, "ARG"), ("H", 0, "SHAPE"),
-    ("H", 3, "SHAPE"), ("max_len", -1, "SHAPE"), ("sinks", -1, "SHAPE"), ("max_new", -1, "SHAPE"), ("q", ODD, "ALIGN"),
+    ("H", 3, "SHAPE"), ("max_len", -1, "SHAPE"), ("sinks", -1, "SHAPE"), ("max_new", -1, "SHAPE"), ("max_new", (1 << 29) + 1, "SHAPE"),
+    ("q", ODD, "ALIGN"),
     ("out", ODD, "ALIGN"), ("q_tok", 12, "ALIGN"), ("q_head", 4, "ALIGN")])
 def test_attention_refuses(arg, value, code):
     from uwc_b200 import _lib
