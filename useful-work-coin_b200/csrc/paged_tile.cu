@@ -19,8 +19,10 @@
 // O stays in TMEM; it is rescaled only when a row's maximum grew by more than 2^4 (so a weight is
 // below 1024 * 2^4 * 2 in fp16, and keeps its 11 bits down to 2^-24 of the reference) or the tile's largest value
 // scale left [1/64, 2] of the reference; both are rare after an item's first tile.
-// Items lie on one line of key tiles, cut into equal parts, one per SM, as in the few-row form; an item in
-// several parts is joined by the last of them in key order.
+// Items lie on one line, cut into equal parts, one per SM, as in the few-row form; an item in several parts is
+// joined by the last of them in key order. An item is as long as its key tiles and kItemCost = 3 more, for its
+// queries, its output and its masked last tiles (about 12,000 cycles to a tile's 4,800; equal numbers of tiles
+// left the SMs with many short items a sixth longer: 8 prompts of 2048 took 236 us instead of 215).
 #include <algorithm>
 
 #include "det_math.cuh"
@@ -42,6 +44,7 @@ constexpr int kPageRing = 8;                 // slots: those, and up to four tha
 constexpr int kSeqs = 1024;                  // sequences whose span and tiles are kept in shared memory
 constexpr int kSmem = 1024 + 6 * kOperand + kSeqs * 24;   // two query tiles, two stages of keys, two of values
 constexpr int kMinTiles = 4;                 // a CTA's least share of the line
+constexpr int kItemCost = 3;                 // what an item costs beside its tiles, in tiles
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 // 128 dims; values are stored key by key: B is MN-major
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(kHd >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
@@ -79,7 +82,7 @@ struct Batch {
     const int nb = blocks(z);
     long long t = 0;
 #pragma unroll 1
-    for (int b = threadIdx.x & 31; b < nb; b += 32) t += Item(a, z, G, b).total;
+    for (int b = threadIdx.x & 31; b < nb; b += 32) t += kItemCost + Item(a, z, G, b).total;
     return warp_sumll(t);
   }
   __device__ __forceinline__ long long tiles(int s) const { return s < kSeqs ? tiles_[s] : count(span(s)); }
@@ -104,9 +107,10 @@ struct Batch {
   }
 };
 
-// A CTA's part of the line of key tiles: `left` tiles from tile t0 of block blk of KV head h of sequence s on.
+// A CTA's part of the line: `left` units from unit u0 of block blk of KV head h of sequence s on. An item's units
+// are kItemCost for itself and one a key tile.
 struct Start {
-  int s, h, blk, t0;
+  int s, h, blk, u0;
   int left, per;
 };
 // One warp, all lanes together.
@@ -135,7 +139,7 @@ __device__ __forceinline__ Start find_start(const Batch& q) {
       for (; rest >= one; p.h++) rest -= one;
 #pragma unroll 1
       for (int b0 = 0; b0 < blks; b0 += 32) {
-        const int t = b0 + lane < blks ? Item(q.a, sp, q.G, b0 + lane).total : 0;
+        const int t = b0 + lane < blks ? kItemCost + Item(q.a, sp, q.G, b0 + lane).total : 0;
         int inc = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -146,7 +150,7 @@ __device__ __forceinline__ Start find_start(const Batch& q) {
         if (hit) {
           const int l = __ffs(hit) - 1;
           p.blk = b0 + l;
-          p.t0 = (int)(rest - __shfl_sync(0xffffffffu, inc - t, l));
+          p.u0 = (int)(rest - __shfl_sync(0xffffffffu, inc - t, l));
           return p;
         }
         rest -= __shfl_sync(0xffffffffu, inc, 31);
@@ -689,50 +693,50 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         const int slot = n % kPieces;
         if (n >= kPieces) TILE_WAIT(bar.piece_empty[slot], (n / kPieces - 1) & 1);
         Piece& k = s_piece[slot];
-        int done = 0;
-        if (p.left > 0) {
+        bool end = true;
+#pragma unroll 1
+        while (p.left > 0 && end) {
           const Item it(a, sp, G, p.blk);
-          const int t1 = min(it.total, p.t0 + p.left);
-          done = t1 - p.t0;
-          if (lane == 0) {
-            k.first = 2 * kRows * p.blk;
-            k.rows = min(2 * kRows, sp.n * G - 2 * kRows * p.blk);
-            k.row0 = sp.row0;
-            k.seq = p.s;
-            k.head = p.h;
-            k.start = sp.idle ? -1 : sp.start;
-            k.t0 = p.t0;
-            k.t1 = t1;
-            k.whole = done == it.total;
-            // the CTAs before this one hold t0 of the item's tiles, those after it the rest, `per` each
-            if (done < it.total) {
-              k.b0 = blockIdx.x - (p.t0 > 0 ? (uint32_t)(p.t0 - 1) / (uint32_t)p.per + 1 : 0);
-              k.b1 = blockIdx.x + (it.total > t1 ? (uint32_t)(it.total - t1 - 1) / (uint32_t)p.per + 1 : 0);
+          const int all = kItemCost + it.total, u1 = min(all, p.u0 + p.left);
+          if (u1 > kItemCost) {                    // some of its tiles, not only its own cost
+            end = false;
+            if (lane == 0) {
+              k.first = 2 * kRows * p.blk;
+              k.rows = min(2 * kRows, sp.n * G - 2 * kRows * p.blk);
+              k.row0 = sp.row0;
+              k.seq = p.s;
+              k.head = p.h;
+              k.start = sp.idle ? -1 : sp.start;
+              k.t0 = max(p.u0 - kItemCost, 0);
+              k.t1 = u1 - kItemCost;
+              k.whole = p.u0 <= kItemCost && u1 == all;
+              // the CTAs before this one hold the item's tiles before t0, those after it the rest, `per` each
+              k.b0 = blockIdx.x - (p.u0 > kItemCost ? (uint32_t)(p.u0 - kItemCost - 1) / (uint32_t)p.per + 1 : 0);
+              k.b1 = blockIdx.x + (all > u1 ? (uint32_t)(all - u1 - 1) / (uint32_t)p.per + 1 : 0);
+              k.lo = it.lo;
+              k.hi = it.hi;
+              k.sink_end = it.sink_end;
+              k.tA = it.tA;
+              k.tB0 = it.tB0;
             }
-            k.lo = it.lo;
-            k.hi = it.hi;
-            k.sink_end = it.sink_end;
-            k.tA = it.tA;
-            k.tB0 = it.tB0;
           }
-        } else if (lane == 0) {
-          k.rows = 0;
+          p.left -= u1 - p.u0;
+          p.u0 = 0;
+          if (p.left > 0 && ++p.blk == blks) {
+            p.blk = 0;
+            if (++p.h == Hkv) {
+              p.h = 0;
+              do {
+                sp = batch.span(++p.s);
+                blks = batch.blocks(sp);
+              } while (blks == 0 && p.s + 1 < a.b.seqs);
+            }
+          }
         }
+        if (end && lane == 0) k.rows = 0;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.piece_full[slot]);
-        if (done == 0) break;
-        p.left -= done;
-        p.t0 = 0;
-        if (p.left > 0 && ++p.blk == blks) {
-          p.blk = 0;
-          if (++p.h == Hkv) {
-            p.h = 0;
-            do {
-              sp = batch.span(++p.s);
-              blks = batch.blocks(sp);
-            } while (blks == 0 && p.s + 1 < a.b.seqs);
-          }
-        }
+        if (end) break;
       }
     } else if (warp == 14) {
       // ---------------------------------------------------------------- the pages: a lane a 16-key group, four tiles at once
