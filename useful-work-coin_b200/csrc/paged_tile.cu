@@ -357,20 +357,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
     // Row x of an item is token (x + rem) / G past the item's first one: a division of small numbers, exact in
     // float32 while they are below 2^20.
     auto token_of = [&](int x) { return (int)(((float)x + 0.5f) * inv_g); };
+    const int dt = 2 / G, dh = 2 - dt * G;         // two rows on: tokens and heads of the group
+    const long long by = dt * a.q_tok + dh * a.q_head, carry = a.q_tok - G * a.q_head;
     // Sends a piece's query rows on their way to this warp's part of the operand, two rows a step.
     auto fetch_q = [&](const Piece& k) {
       const int rows = min(kRows, k.rows - kRows * w);
       if (rows <= 0) return;
-      const int tok0 = k.first / G, y = kRows * w + r + k.first - tok0 * G, tok = token_of(y), head = y - tok * G, c = lane & 15;
-      const T* q = reinterpret_cast<const T*>(a.q) + (long long)(k.row0 + tok0) * a.q_tok + (long long)(k.head * G) * a.q_head + 8 * c;
-      const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf;
-#pragma unroll 2
-      for (int i = 0; i < 16; i++) {
-        const int x = 2 * i + (lane >> 4), rr = 32 * (warp & 3) + x;
-        const int tk = __shfl_sync(0xffffffffu, tok, x), hd = __shfl_sync(0xffffffffu, head, x);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)),
-                     "l"(rr < rows ? q + tk * a.q_tok + hd * a.q_head : q), "r"(rr < rows ? 16 : 0)
+      const int r0 = 32 * (warp & 3) + (lane >> 4), tok = token_of(k.first - k.first / G * G + kRows * w + r0), c = lane & 15;
+      int head = k.first - k.first / G * G + kRows * w + r0 - tok * G;
+      const T* q = reinterpret_cast<const T*>(a.q) + (long long)(k.row0 + k.first / G + tok) * a.q_tok + (long long)(k.head * G + head) * a.q_head + 8 * c;
+      const uint32_t at = smQ + w * kOperand + (c >> 3) * kHalf + r0 * 128;
+#pragma unroll 4
+      for (int x = 0; x < 32; x += 2) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + x * 128 + (((c & 7) ^ ((r0 + x) & 7)) << 4)),
+                     "l"(r0 + x < rows ? q : reinterpret_cast<const T*>(a.q)), "r"(r0 + x < rows ? 16 : 0)
                      : "memory");
+        q += by;
+        head += dh;
+        if (head >= G) {
+          head -= G;
+          q += carry;
+        }
       }
     };
     TILE_WAIT(bar.piece_full[0], 0);
