@@ -10,7 +10,10 @@
 // bound is the cache's bytes from HBM. The visible keys of all (sequence, KV head) units, in tiles of 64,
 // form one line that is cut into equal parts, one per resident CTA: any raggedness is balanced, and a
 // unit that lies in several parts is joined by the last CTA to finish it, in key order, so the bits do
-// not depend on which that is. Per CTA one warp fetches pages (TMA, 128-byte swizzle, a ring of 16 KiB
+// not depend on which that is. A unit is kUnitCost tiles longer than its keys, for its queries, its four
+// warps' sums and its output: with equal numbers of tiles the CTAs with many short units ended last (32
+// sequences of 1 to 8192, 32 heads on 8: 71.7 us; with 3, 5 and 8 tiles a unit 59.4, 59.2 and 58.5; 16
+// sequences with 4 drafts each 32.4, 27.5, 26.7 and 27.3). Per CTA one warp fetches pages (TMA, 128-byte swizzle, a ring of 16 KiB
 // stages, page ids and scales eight tiles ahead) and four warps compute, 16 keys of a tile each:
 //   S^T = K Q^T and O^T = V^T P^T as mma m16n8k16 in fp16 with float32 sums. The integers are exact in
 //   fp16 (a byte permute and one subtraction a pair); a query row is scaled by a power of two that puts
@@ -39,7 +42,8 @@ constexpr int kTile = 64;                    // keys per stage
 constexpr int kGroups = kTile / 16;          // 16-key groups: one warp's share, always inside one page
 constexpr int kStageBytes = 2 * kTile * kHd; // keys, then values
 constexpr int kBatch = 8;                    // tiles whose page ids and scales are fetched at once
-constexpr int kMinTiles = 4;                 // a CTA's least share of the line (a join costs about as much)
+constexpr int kUnitCost = 5;                 // what a unit costs beside its tiles, in tiles
+constexpr int kMinTiles = 4;                 // the least tiles of a CTA's share of the line (a join costs about as much)
 
 // rows: 8 NT. Stages and CTAs per SM: about 200 KB of loads in flight on an SM either way.
 template <int NT>
@@ -63,13 +67,15 @@ struct Unit : Keys<kTile> {
   __device__ __forceinline__ Unit(const AttnArgs& a, const Span& s) : Keys<kTile>(a, s, 0, s.n - 1), sp(s) {
     if (s.n <= 0) total = 0;
   }
+  __device__ __forceinline__ int cost() const { return total > 0 ? kUnitCost + total : 0; }   // its length on the line
 };
 __device__ __forceinline__ Unit unit_of(const AttnArgs& a, int s) { return Unit(a, span_of(a.b, a.c.ps, s)); }
 
-// This CTA's part of the line: `count` tiles from tile `tile` of KV head `head` of sequence `seq` on.
+// This CTA's part of the line: `count` steps from step `at` of KV head `head` of sequence `seq` on. A unit's steps
+// are kUnitCost for itself, then one a tile.
 struct Part {
-  int seq, head, tile;
-  long long first, per, total;     // of the line, in tiles
+  int seq, head, at;
+  uint32_t per;                    // steps of a part (2^32 of them would be days of work)
   long long count;
 };
 // Every warp finds it for itself: lanes take sequences, two passes (the sum, then the place).
@@ -79,36 +85,36 @@ __device__ __forceinline__ Part find_part(const AttnArgs& a) {
   int most = 0;
 #pragma unroll 1
   for (int s = lane; s < S; s += 32) {
-    const int t = unit_of(a, s).total;
+    const int t = unit_of(a, s).cost();
     sum += t;
     most = max(most, t);
   }
   sum = warp_sumll(sum);
   most = __reduce_max_sync(0xffffffffu, most);
   Part p = {};
-  p.total = sum * a.c.Hkv;
-  p.per = max((p.total + gridDim.x - 1) / gridDim.x, (long long)min(kMinTiles, most));
-  p.first = p.per * blockIdx.x;
-  p.count = min(p.per, p.total - p.first);
+  sum *= a.c.Hkv;
+  p.per = (uint32_t)max((sum + gridDim.x - 1) / gridDim.x, (long long)min(kMinTiles + kUnitCost, most));
+  const long long first = (long long)p.per * blockIdx.x;
+  p.count = min((long long)p.per, sum - first);
   if (p.count <= 0) return p;
   long long before = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < S; s0 += 32) {
-    const long long t = s0 + lane < S ? (long long)unit_of(a, s0 + lane).total * a.c.Hkv : 0;
+    const long long t = s0 + lane < S ? (long long)unit_of(a, s0 + lane).cost() * a.c.Hkv : 0;
     long long inc = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > p.first);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > first);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      const long long at = p.first - (before + __shfl_sync(0xffffffffu, inc - t, l));
-      const int tiles = (int)(__shfl_sync(0xffffffffu, t, l) / a.c.Hkv);
+      const long long at = first - (before + __shfl_sync(0xffffffffu, inc - t, l));
+      const int steps = (int)(__shfl_sync(0xffffffffu, t, l) / a.c.Hkv);
       p.seq = s0 + l;
-      p.head = (int)(at / tiles);
-      p.tile = (int)(at % tiles);
+      p.head = (int)(at / steps);
+      p.at = (int)(at % steps);
       return p;
     }
     before += __shfl_sync(0xffffffffu, inc, 31);
@@ -174,14 +180,14 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
     const int box = min(ps, kTile), per_box = box / 16;      // keys, 16-key groups a TMA box
     const int grp = lane & (kGroups - 1);
     int it = 0;
-    int s = part.seq, h = part.head, t0 = part.tile;
+    int s = part.seq, h = part.head, u0 = part.at;
     long long left = part.count;
 #pragma unroll 1
     while (left > 0) {
       const Unit k = unit_of(a, s);
 #pragma unroll 1
-      for (; h < Hkv && t0 < k.total && left > 0;) {
-        const int end = (int)min((long long)k.total, t0 + left);
+      for (; h < Hkv && left > 0; h++, u0 = 0) {
+        const int u1 = (int)min((long long)k.cost(), u0 + left), t0 = max(u0 - kUnitCost, 0), end = u1 - kUnitCost;
         // page ids and scales of eight tiles, one 16-key group a lane
         auto fetch = [&](int tb, int& page, float2& sc, int& j0) {
           const int i = tb + lane / kGroups;
@@ -194,9 +200,9 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
             else sc = make_float2(a.c.sk[(size_t)page * Hkv + h], a.c.sv[(size_t)page * Hkv + h]);
           }
         };
-        int page, j0, npage = -1, nj0 = 0;
-        float2 sc, nsc = make_float2(0.f, 0.f);
-        fetch(t0, page, sc, j0);
+        int page = -1, j0 = 0, npage = -1, nj0 = 0;
+        float2 sc = make_float2(0.f, 0.f), nsc = sc;
+        if (end > t0) fetch(t0, page, sc, j0);
 #pragma unroll 1
         for (int tb = t0; tb < end; tb += kBatch) {
           if (tb + kBatch < end) fetch(tb + kBatch, npage, nsc, nj0);
@@ -239,17 +245,11 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           sc = nsc;
           j0 = nj0;
         }
-        left -= end - t0;
-        if (end == k.total) {
-          h++;
-          t0 = 0;
-        } else {
-          t0 = end;
-        }
+        left -= u1 - u0;
       }
       s++;
       h = 0;
-      t0 = 0;
+      u0 = 0;
 #pragma unroll 1
       while (left > 0 && s < a.b.seqs && unit_of(a, s).total == 0) s++;
       if (s >= a.b.seqs) break;
@@ -265,15 +265,17 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
   const uint32_t voff0 = kTile * kHd + (16 * warp + 2 * t) * kHd + ((g ^ (2 * t)) << 4);
   const uint32_t voff1 = kTile * kHd + (16 * warp + 2 * t + 1) * kHd + ((g ^ (2 * t + 1)) << 4);
   int it = 0;
-  int s = part.seq, h = part.head, t0 = part.tile;
-  long long left = part.count, at = part.first;      // at: the line's tile that t0 is
+  int s = part.seq, h = part.head, u0 = part.at;
+  long long left = part.count;
 #pragma unroll 1
   while (left > 0) {
     const Unit k = unit_of(a, s);
     const int rows = k.sp.n * G;
 #pragma unroll 1
-    for (; h < Hkv && left > 0; h++, t0 = 0) {
-      const int end = (int)min((long long)k.total, t0 + left);
+    for (; h < Hkv && left > 0; h++, u0 = 0) {
+      const int u1 = (int)min((long long)k.cost(), u0 + left), t0 = max(u0 - kUnitCost, 0), end = u1 - kUnitCost;
+      left -= u1 - u0;
+      if (end <= t0) continue;                           // none of its tiles
       // ---- this unit's queries: row r = token r / G, head r % G; thread (g, t) has dims 32 t .. of rows g + 8 n
       uint32_t qf[NT][8][2];
       float qmul[NT][2];
@@ -504,15 +506,20 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
               o[n][d][2 + c] += x.y;
             }
       };
-      if (warp >= 2) put(comb + (warp - 2) * R * kHd);
-      named_bar_sync(1, kWarps * 32);
-      if (warp < 2) add(comb + warp * R * kHd);
-      if (warp == 1) put(comb + R * kHd);      // its own region: only this warp read it
-      named_bar_sync(1, kWarps * 32);
+      // onto warp 0, one warp after the other (a rolled loop: a CTA comes here once or twice, and straight-line
+      // code would be fetched for as long as it runs)
+#pragma unroll 1
+      for (int w = 1; w <= kWarps; w++) {
+        if (warp == w) put(comb + (w & 1) * R * kHd);
+        if (warp == 0 && w > 1) add(comb + ((w - 1) & 1) * R * kHd);
+        named_bar_sync(1, kWarps * 32);
+      }
       const bool whole = t0 == 0 && end == k.total;
-      const long long u0 = at - t0;             // the unit's first tile on the line
+      // parts of this unit lie in CTAs b0 .. b1: its tiles before t0 in those before this one, `per` steps each,
+      // those from `end` on in those after it
+      const int b0 = blockIdx.x - (t0 > 0 ? (uint32_t)(t0 - 1) / part.per + 1 : 0);
+      const int b1 = blockIdx.x + (end < k.total ? (uint32_t)(k.total - end - 1) / part.per + 1 : 0);
       if (warp == 0) {
-        add(comb + R * kHd);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -543,8 +550,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
             }
           }
         if (!whole) {
-          // parts of this unit lie in CTAs b0 .. b1; the last of them to get here joins them
-          const int b0 = (int)(u0 / part.per), b1 = (int)((u0 + k.total - 1) / part.per);
+          // the last of this unit's CTAs to get here joins its parts
           __threadfence();
           __syncwarp();
           if (lane == 0) {
@@ -558,27 +564,43 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
       if (!whole) {
         named_bar_sync(1, kWarps * 32);
         if (s_last) {
-          const int b0 = (int)(u0 / part.per), b1 = (int)((u0 + k.total - 1) / part.per);
           __threadfence();
 #pragma unroll 1
           for (int r = warp; r < rows; r += kWarps) {
             auto slot = [&](int b) { return (size_t)(2 * b + (b == b0)) * R + r; };
             float M = kNoMax, L = 0.f;
-#pragma unroll 1
-            for (int b = b0 + lane; b <= b1; b += 32) M = fmaxf(M, __ldcg(&ta.part_ml[slot(b)]).x);
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int b = b0; b <= b1; b++) {
-              const float2 ml = __ldcg(&ta.part_ml[slot(b)]);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(ta.part_o + slot(b) * kHd) + lane);
-              const float f = exp2_fast(ml.x - M);
-              L = fmaf(ml.y, f, L);
-              acc.x = fmaf(x.x, f, acc.x);
-              acc.y = fmaf(x.y, f, acc.y);
-              acc.z = fmaf(x.z, f, acc.z);
-              acc.w = fmaf(x.w, f, acc.w);
+            // one pass, eight parts' loads in flight (a part past b1 loads b1's again and counts nothing)
+#pragma unroll 1
+            for (int b = b0; b <= b1; b += 8) {
+              float2 ml[8];
+              float4 x[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const size_t at = slot(min(b + i, b1));
+                ml[i] = __ldcg(&ta.part_ml[at]);
+                x[i] = __ldcg(reinterpret_cast<const float4*>(ta.part_o + at * kHd) + lane);
+              }
+              float M2 = M;
+#pragma unroll
+              for (int i = 0; i < 8; i++) M2 = fmaxf(M2, ml[i].x);
+              const float down = exp2_fast(M - M2);
+              M = M2;
+              L *= down;
+              acc.x *= down;
+              acc.y *= down;
+              acc.z *= down;
+              acc.w *= down;
+#pragma unroll
+              for (int i = 0; i < 8; i++)
+                if (b + i <= b1) {
+                  const float f = exp2_fast(ml[i].x - M);
+                  L = fmaf(ml[i].y, f, L);
+                  acc.x = fmaf(x[i].x, f, acc.x);
+                  acc.y = fmaf(x[i].y, f, acc.y);
+                  acc.z = fmaf(x[i].z, f, acc.z);
+                  acc.w = fmaf(x[i].w, f, acc.w);
+                }
             }
             const float inv = L == 0.f ? 0.f : 1.f / L;
             T* out = reinterpret_cast<T*>(a.out) + ((size_t)(k.sp.row0 + r / G) * a.H + h * G + r % G) * kHd + 4 * lane;
@@ -586,13 +608,10 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           }
         }
       }
-      at += end - t0;
-      left -= end - t0;
-      if (left <= 0) break;
     }
     s++;
     h = 0;
-    t0 = 0;
+    u0 = 0;
 #pragma unroll 1
     while (left > 0 && s < a.b.seqs && unit_of(a, s).total == 0) s++;
     if (s >= a.b.seqs) break;
