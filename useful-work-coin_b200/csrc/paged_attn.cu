@@ -21,8 +21,9 @@
 //   1/sqrt(d) multiply the float32 sums. Keys lie on the M side, so the conversion serves every query
 //   row, and the order of dims and keys inside a fragment is chosen so that a thread reads 16-byte runs
 //   (conflict-free under the swizzle) and no shuffle moves K or V; P is transposed by movmatrix.
-//   The running maximum is raised only when a score passes it by 2^8 (the weights stay below 256, far
-//   inside fp16), so most tiles neither reduce over lanes nor rescale.
+//   Weights are 2^(score - m) with m 7 below the row's maximum when it was last looked at; m is raised only
+//   when a score passes it by 15, so most tiles neither reduce over lanes nor rescale. They stay below 2^15,
+//   inside fp16, which keeps 11 bits of those down to 2^-21 of the largest (2^-14 without the 7).
 #include <algorithm>
 #include <mutex>
 #include <set>
@@ -41,6 +42,7 @@ constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kTile = 64;                    // keys per stage
 constexpr int kGroups = kTile / 16;          // 16-key groups: one warp's share, always inside one page
 constexpr int kStageBytes = 2 * kTile * kHd; // keys, then values
+constexpr float kHeadroom = 7.f, kRaise = 8.f;   // log2: of the largest weight when m is set; by which a later one may pass it
 constexpr int kBatch = 8;                    // tiles whose page ids and scales are fetched at once
 constexpr int kUnitCost = 5;                 // what a unit costs beside its tiles, in tiles
 constexpr int kMinTiles = 4;                 // the least tiles of a CTA's share of the line (a join costs about as much)
@@ -57,7 +59,7 @@ struct TokenCfg {
 struct TokenArgs {
   AttnArgs a;
   float* part_o;           // (2 grid, 8 NT, 128): a CTA's two partial units, unnormalized
-  float2* part_ml;         // (2 grid, 8 NT): running maximum (log2), sum
+  float2* part_ml;         // (2 grid, 8 NT): m (log2), sum
   uint32_t* counters;      // (grid): finished parts of the unit that starts in this CTA; left zero
 };
 
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) over |= sa[n][x] > m[n][x & 1] + 8.f;
+            for (int x = 0; x < 4; x++) over |= sa[n][x] > m[n][x & 1] + (kHeadroom + kRaise);
           if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                x = fmaxf(x, m[n][c]);
+                x = fmaxf(x - kHeadroom, m[n][c]);
                 const float f = exp2_fast(m[n][c] - x);
                 m[n][c] = x;
                 l[n][c] *= f;
