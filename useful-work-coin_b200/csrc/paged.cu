@@ -316,12 +316,13 @@ __device__ __forceinline__ void requantize(const PageUnit& u, float s0, float s,
 // packed (16 bits); without a norm a key is rotated twice, for the maximum and for its quantization, which
 // costs less than the registers that would hold it: at 64 registers instead of 86 the SM has four CTAs'
 // loads in flight, not two (8 x 2048 tokens of 16 + 2 x 8 heads: 66 us, 121 us before).
-template <typename T, int NP, bool NORM>
-__global__ void __launch_bounds__(kThreads, NORM ? 2 : NP == 4 ? 3 : 4) k_paged_append(const AppendArgs a) {
+// Pages of 16 have CTAs of half the size: half of 256 threads had no row.
+template <typename T, int NP, int TH, bool NORM>
+__global__ void __launch_bounds__(TH, (NORM ? 2 : NP == 4 ? 3 : 4) * kThreads / TH) k_paged_append(const AppendArgs a) {
   const int tid = threadIdx.x, c = tid & 7, r8 = tid >> 3;
   const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
   if (blockIdx.x >= units) {
-    query_unit<T, NORM>(a, (blockIdx.x - units) * (kThreads / 8) + r8, c);
+    query_unit<T, NORM>(a, (blockIdx.x - units) * (TH / 8) + r8, c);
     return;
   }
   PageUnit u;
@@ -330,31 +331,31 @@ __global__ void __launch_bounds__(kThreads, NORM ? 2 : NP == 4 ? 3 : 4) k_paged_
   Raw raw[NP];
 #pragma unroll
   for (int n = 0; n < NP; n++) {
-    const int p = u.base + n * 32 + r8;
+    const int p = u.base + n * (TH / 8) + r8;
     raw[n] = Raw{};
     if (p >= u.p0 && p < u.p1) raw[n] = load_raw<T>(u.is_k ? a.k : a.v, u.row0 + p, u.h, c);
   }
   float amax = 0.f;
 #pragma unroll
   for (int n = 0; n < NP; n++) {
-    const int p = u.base + n * 32 + r8;
+    const int p = u.base + n * (TH / 8) + r8;
     const bool live = p >= u.p0 && p < u.p1;
     float lo[8], hi[8];
     row_values<T, NORM>(a, u, raw[n], p, live, c, lo, hi);
     if (live) amax = fmaxf(amax, row_max(lo, hi));
   }
-  __shared__ float red[kThreads / 32];
-  amax = block_maxf<kThreads>(amax, red);
+  __shared__ float red[TH / 32];
+  amax = block_maxf<TH>(amax, red);
   const float sn = fmaxf(s0, __fdiv_rn(amax, 127.0f)), inv = inverse(sn);
 #pragma unroll
   for (int n = 0; n < NP; n++) {
-    const int p = u.base + n * 32 + r8;
+    const int p = u.base + n * (TH / 8) + r8;
     const bool live = p >= u.p0 && p < u.p1;
     float lo[8], hi[8];
     row_values<T, NORM>(a, u, raw[n], p, live, c, lo, hi);
     if (live) store_row(u, p, c, lo, hi, sn, inv);
   }
-  if (u.p0 > u.base && sn > s0) requantize(u, s0, sn, inv, tid, kThreads);
+  if (u.p0 > u.base && sn > s0) requantize(u, s0, sn, inv, tid, TH);
   if (tid == 0) *u.scale = sn;   // after block_maxf's barriers: every thread has read s0
 }
 
@@ -470,12 +471,14 @@ int launch_append(const AppendArgs& a, cudaStream_t st) {
   const long long queries = a.q.p ? (long long)a.b.rows * ((a.H + kQHeads - 1) / kQHeads) : 0;
   const bool few = a.b.max_new <= kFewNew;
   const long long per = kFewThreads / 32;
-  const long long grid = few ? (units + (queries + 3) / 4 + per - 1) / per : units + (queries * 8 + kThreads - 1) / kThreads;
+  const int threads = a.c.ps == 16 ? kThreads / 2 : kThreads;
+  const long long grid = few ? (units + (queries + 3) / 4 + per - 1) / per : units + (queries * 8 + threads - 1) / threads;
   if (grid > 0x7fffffffll) return UWC_ERR_SHAPE;
   if (few) k_paged_append_few<T, NORM><<<(unsigned)grid, kFewThreads, 0, st>>>(a);
-  else if (a.c.ps == 128) k_paged_append<T, 4, NORM><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else if (a.c.ps == 64) k_paged_append<T, 2, NORM><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else k_paged_append<T, 1, NORM><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  else if (a.c.ps == 128) k_paged_append<T, 4, kThreads, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
+  else if (a.c.ps == 64) k_paged_append<T, 2, kThreads, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
+  else if (a.c.ps == 32) k_paged_append<T, 1, kThreads, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
+  else k_paged_append<T, 1, kThreads / 2, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
   uwc_count_launch();
   return uwc_launch_status();
 }
