@@ -142,18 +142,18 @@ __device__ __forceinline__ uint32_t quant4_exact(float4 x4, float s) {
 // The same without the divisions (half of the kernel's instructions) where that cannot change a bit: inv is
 // 1 / s, so x inv is within 1e-4 of the quotient (|quotient| <= 127), and both round to the same integer
 // unless it lies that near to a half. 1.5 2^23 + x inv has the integer in its low byte. Infinities, NaN and
-// an infinite inv fail the test too.
+// an infinite inv leave a NaN, which fails the test too.
 __device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv) {
   constexpr float kMagic = 12582912.f;
   uint32_t t[4];
-  bool sure = true;
+  float off = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const float y = x[i] * inv, z = y + kMagic;
+    const float z = fmaf(x[i], inv, kMagic);
     t[i] = __float_as_uint(z);
-    sure = sure && fabsf(y - (z - kMagic)) < 0.4999f;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(fmaf(x[i], inv, kMagic - z))));
   }
-  if (!sure) return quant4_exact(make_float4(x[0], x[1], x[2], x[3]), s);
+  if (!(off < 0.4999f)) return quant4_exact(make_float4(x[0], x[1], x[2], x[3]), s);
   return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 __device__ __forceinline__ float inverse(float s) { return s > 1e-30f ? __frcp_rn(s) : __int_as_float(0x7f800000); }
@@ -240,17 +240,19 @@ __device__ __forceinline__ void query_unit(const AppendArgs& a, long long u, int
       }
 }
 
-// A page's part in a call: unit (sequence, touched page, KV head, keys or values).
+// A page's part in a call: unit (sequence, touched page, HP KV heads, keys or values).
 struct PageUnit {
-  int p0, p1, base, row0, h;   // positions p0 .. p1 - 1 are written; row of position p: row0 + p
+  int p0, p1, base, row0, h;   // positions p0 .. p1 - 1 are written; row of position p: row0 + p; first head
   bool is_k;
   int8_t* data;                // the page's (page_size, 128) of the head
   float* scale;
 };
+template <int HP = 1>
 __device__ __forceinline__ bool page_unit(const AppendArgs& a, long long unit, bool leader, PageUnit& u) {
+  const int parts = (a.c.Hkv + HP - 1) / HP;
   u.is_k = (unit & 1) == 0;
-  u.h = (int)((unit >> 1) % a.c.Hkv);
-  const int sj = (int)((unit >> 1) / a.c.Hkv), s = sj / a.most, j = sj - s * a.most;
+  u.h = (int)((unit >> 1) % parts) * HP;
+  const int sj = (int)((unit >> 1) / parts), s = sj / a.most, j = sj - s * a.most;
   const Span sp = span_of(a.b, a.c.ps, s);
   if (sp.bad && j == 0 && leader) set_status(a.status, UWC_DEV_RANGE);
   if (sp.idle || sp.n <= 0) return false;
@@ -312,51 +314,124 @@ __device__ __forceinline__ void requantize(const PageUnit& u, float s0, float s,
   }
 }
 
-// Prompts: one CTA a page unit, its rows in NP passes of 32. All rows' loads are issued first and stay
-// packed (16 bits); without a norm a key is rotated twice, for the maximum and for its quantization, which
-// costs less than the registers that would hold it: at 64 registers instead of 86 the SM has four CTAs'
-// loads in flight, not two (8 x 2048 tokens of 16 + 2 x 8 heads: 66 us, 121 us before).
-// Pages of 16 have CTAs of half the size: half of 256 threads had no row.
-template <typename T, int NP, int TH, bool NORM>
-__global__ void __launch_bounds__(TH, (NORM ? 2 : NP == 4 ? 3 : 4) * kThreads / TH) k_paged_append(const AppendArgs a) {
+// Four of a lane's low and of its high values.
+template <typename T>
+__device__ __forceinline__ void unpack4(const Raw& r, int k, float* lo, float* hi) {
+  const uint32_t* l = reinterpret_cast<const uint32_t*>(&r.lo) + 2 * k;
+  const uint32_t* h = reinterpret_cast<const uint32_t*>(&r.hi) + 2 * k;
+  const float2 a = paged::two_f(l[0], T()), b = paged::two_f(l[1], T()), c = paged::two_f(h[0], T()), d = paged::two_f(h[1], T());
+  lo[0] = a.x, lo[1] = a.y, lo[2] = b.x, lo[3] = b.y;
+  hi[0] = c.x, hi[1] = c.y, hi[2] = d.x, hi[3] = d.y;
+}
+
+// Prompts: one CTA a page unit of HP heads, its rows in NP passes of TH / 8. All rows' loads are issued first
+// and stay packed (16 bits); without a norm a key is rotated twice, for the maximum and for its quantization,
+// which costs less than the registers that would hold it: at 64 registers instead of 86 the SM has four CTAs'
+// loads in flight, not two. Two heads share the rotation values, which are four times a key's bytes (13 x up
+// to 777 tokens of 12 + 2 x 4 heads, pages of 16: 13.2 us instead of 15.2). Pages of 16 have CTAs of half the size: half of 256 threads had no row.
+template <typename T, int NP, int TH, int HP, bool NORM>
+__global__ void __launch_bounds__(TH, (NORM ? 2 : NP * HP == 4 ? 3 : 4) * kThreads / TH) k_paged_append(const AppendArgs a) {
   const int tid = threadIdx.x, c = tid & 7, r8 = tid >> 3;
-  const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
+  const long long units = (long long)a.b.seqs * a.most * ((a.c.Hkv + HP - 1) / HP) * 2;
   if (blockIdx.x >= units) {
     query_unit<T, NORM>(a, (blockIdx.x - units) * (TH / 8) + r8, c);
     return;
   }
   PageUnit u;
-  if (!page_unit(a, blockIdx.x, tid == 0, u)) return;
-  const float s0 = u.p0 > u.base ? *u.scale : 0.f;
-  Raw raw[NP];
+  if (!page_unit<HP>(a, blockIdx.x, tid == 0, u)) return;
+  const int heads = min(HP, a.c.Hkv - u.h);
+  float s0[HP];
+  Raw raw[NP][HP];
+#pragma unroll
+  for (int g = 0; g < HP; g++) s0[g] = u.p0 > u.base && g < heads ? u.scale[g] : 0.f;
 #pragma unroll
   for (int n = 0; n < NP; n++) {
     const int p = u.base + n * (TH / 8) + r8;
-    raw[n] = Raw{};
-    if (p >= u.p0 && p < u.p1) raw[n] = load_raw<T>(u.is_k ? a.k : a.v, u.row0 + p, u.h, c);
-  }
-  float amax = 0.f;
 #pragma unroll
-  for (int n = 0; n < NP; n++) {
-    const int p = u.base + n * (TH / 8) + r8;
-    const bool live = p >= u.p0 && p < u.p1;
-    float lo[8], hi[8];
-    row_values<T, NORM>(a, u, raw[n], p, live, c, lo, hi);
-    if (live) amax = fmaxf(amax, row_max(lo, hi));
+    for (int g = 0; g < HP; g++) {
+      raw[n][g] = Raw{};
+      if (p >= u.p0 && p < u.p1 && g < heads) raw[n][g] = load_raw<T>(u.is_k ? a.k : a.v, u.row0 + p, u.h + g, c);
+    }
   }
-  __shared__ float red[TH / 32];
-  amax = block_maxf<TH>(amax, red);
-  const float sn = fmaxf(s0, __fdiv_rn(amax, 127.0f)), inv = inverse(sn);
-#pragma unroll
-  for (int n = 0; n < NP; n++) {
+  // a row's values, four low and four high dims of a head at a time
+  auto each = [&](int n, auto&& f) {
     const int p = u.base + n * (TH / 8) + r8;
     const bool live = p >= u.p0 && p < u.p1;
-    float lo[8], hi[8];
-    row_values<T, NORM>(a, u, raw[n], p, live, c, lo, hi);
-    if (live) store_row(u, p, c, lo, hi, sn, inv);
+    if (NORM) {
+      float lo[8], hi[8];
+      row_values<T, NORM>(a, u, raw[n][0], p, live, c, lo, hi);
+      if (live)
+#pragma unroll
+        for (int k = 0; k < 2; k++) f(0, k, lo + 4 * k, hi + 4 * k);
+    } else if (live) {
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        Turn4 t;
+        if (u.is_k) t = load_turn(a.cos, a.sin, p, c, k);
+#pragma unroll
+        for (int g = 0; g < HP; g++) {
+          float lo[4], hi[4];
+          unpack4<T>(raw[n][g], k, lo, hi);
+          if (u.is_k) rotate4(t, lo, hi);
+          f(g, k, lo, hi);
+        }
+      }
+    }
+  };
+  // the largest magnitudes (a maximum passes NaN over); infinities do not count, and are rare
+  float amax[HP], sn[HP], inv[HP];
+#pragma unroll
+  for (int g = 0; g < HP; g++) amax[g] = 0.f;
+#pragma unroll
+  for (int n = 0; n < NP; n++)
+    each(n, [&](int g, int, const float* lo, const float* hi) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) amax[g] = fmaxf(amax[g], fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+    });
+  __shared__ float red[HP][TH / 32];
+  bool infinite = false;
+#pragma unroll
+  for (int g = 0; g < HP; g++) {
+    amax[g] = block_maxf<TH>(amax[g], red[g]);
+    infinite |= amax[g] > FLT_MAX;
   }
-  if (u.p0 > u.base && sn > s0) requantize(u, s0, sn, inv, tid, TH);
-  if (tid == 0) *u.scale = sn;   // after block_maxf's barriers: every thread has read s0
+  if (infinite) {
+    __syncthreads();                               // red is used again
+#pragma unroll
+    for (int g = 0; g < HP; g++) amax[g] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NP; n++)
+      each(n, [&](int g, int, const float* lo, const float* hi) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) amax[g] = fmaxf(amax[g], fmaxf(finite_abs(lo[i]), finite_abs(hi[i])));
+      });
+#pragma unroll
+    for (int g = 0; g < HP; g++) amax[g] = block_maxf<TH>(amax[g], red[g]);
+  }
+#pragma unroll
+  for (int g = 0; g < HP; g++) {
+    sn[g] = fmaxf(s0[g], __fdiv_rn(amax[g], 127.0f));
+    inv[g] = inverse(sn[g]);
+  }
+  const size_t head = (size_t)a.c.ps * kHd;
+#pragma unroll
+  for (int n = 0; n < NP; n++) {
+    int8_t* d = u.data + (size_t)(n * (TH / 8) + r8) * kHd + 8 * c;
+    each(n, [&](int g, int k, const float* lo, const float* hi) {
+      if (g < heads) {
+        *reinterpret_cast<uint32_t*>(d + g * head + 4 * k) = quant4(lo, sn[g], inv[g]);
+        *reinterpret_cast<uint32_t*>(d + g * head + 4 * k + 64) = quant4(hi, sn[g], inv[g]);
+      }
+    });
+  }
+#pragma unroll
+  for (int g = 0; g < HP; g++)
+    if (g < heads) {
+      PageUnit v = u;
+      v.data += g * head;
+      if (u.p0 > u.base && sn[g] > s0[g]) requantize(v, s0[g], sn[g], inv[g], tid, TH);
+      if (tid == 0) u.scale[g] = sn[g];   // after block_maxf's barriers: every thread has read s0
+    }
 }
 
 // Decode steps (at most kFewNew new tokens a sequence): one warp a page unit, so that a batch's units are
@@ -465,22 +540,32 @@ namespace {
 
 bool row_strides_ok(long long tok, long long head) { return tok >= 0 && head >= 0 && tok % 8 == 0 && head % 8 == 0; }
 
-template <typename T, bool NORM>
-int launch_append(const AppendArgs& a, cudaStream_t st) {
-  const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
+template <typename T, int NP, int TH, int HP, bool NORM>
+int launch_pages(const AppendArgs& a, cudaStream_t st) {
+  const long long units = (long long)a.b.seqs * a.most * ((a.c.Hkv + HP - 1) / HP) * 2;
   const long long queries = a.q.p ? (long long)a.b.rows * ((a.H + kQHeads - 1) / kQHeads) : 0;
-  const bool few = a.b.max_new <= kFewNew;
-  const long long per = kFewThreads / 32;
-  const int threads = a.c.ps == 16 ? kThreads / 2 : kThreads;
-  const long long grid = few ? (units + (queries + 3) / 4 + per - 1) / per : units + (queries * 8 + threads - 1) / threads;
+  const long long grid = units + (queries * 8 + TH - 1) / TH;
   if (grid > 0x7fffffffll) return UWC_ERR_SHAPE;
-  if (few) k_paged_append_few<T, NORM><<<(unsigned)grid, kFewThreads, 0, st>>>(a);
-  else if (a.c.ps == 128) k_paged_append<T, 4, kThreads, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
-  else if (a.c.ps == 64) k_paged_append<T, 2, kThreads, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
-  else if (a.c.ps == 32) k_paged_append<T, 1, kThreads, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
-  else k_paged_append<T, 1, kThreads / 2, NORM><<<(unsigned)grid, threads, 0, st>>>(a);
+  k_paged_append<T, NP, TH, HP, NORM><<<(unsigned)grid, TH, 0, st>>>(a);
   uwc_count_launch();
   return uwc_launch_status();
+}
+template <typename T, bool NORM>
+int launch_append(const AppendArgs& a, cudaStream_t st) {
+  if (a.b.max_new <= kFewNew) {
+    const long long units = (long long)a.b.seqs * a.most * a.c.Hkv * 2;
+    const long long queries = a.q.p ? (long long)a.b.rows * ((a.H + kQHeads - 1) / kQHeads) : 0;
+    const long long per = kFewThreads / 32, grid = (units + (queries + 3) / 4 + per - 1) / per;
+    if (grid > 0x7fffffffll) return UWC_ERR_SHAPE;
+    k_paged_append_few<T, NORM><<<(unsigned)grid, kFewThreads, 0, st>>>(a);
+    uwc_count_launch();
+    return uwc_launch_status();
+  }
+  constexpr int HP = NORM ? 1 : 2;                 // a norm holds a whole head's values
+  if (a.c.ps == 128) return launch_pages<T, 4, kThreads, 1, NORM>(a, st);
+  if (a.c.ps == 64) return launch_pages<T, 2, kThreads, HP, NORM>(a, st);
+  if (a.c.ps == 32) return launch_pages<T, 1, kThreads, HP, NORM>(a, st);
+  return launch_pages<T, 1, kThreads / 2, HP, NORM>(a, st);
 }
 
 }  // namespace
