@@ -10,7 +10,9 @@
 //                    and appending the same tokens again changes nothing.
 //   k_paged_gather   cached tokens back as 16- or 32-bit values.
 //
-// Both are bound by HBM at prompt sizes and by latency at decode sizes.
+// Both are bound by HBM at prompt sizes and by latency at decode sizes. Measured on B200 (a graph of calls): 8
+// prompts of 2048, 16 + 2 x 8 heads, 63 us (3.7 TB/s: about 20 instructions a value, twice over the rows) and 20 us
+// to read it back; a token each of 64 sequences, 32 + 2 x 8 heads, 4.8 us.
 #include <cfloat>
 
 #include "det_math.cuh"

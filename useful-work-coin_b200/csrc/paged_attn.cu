@@ -24,6 +24,11 @@
 //   Weights are 2^(score - m) with m 7 below the row's maximum when it was last looked at; m is raised only
 //   when a score passes it by 15, so most tiles neither reduce over lanes nor rescale. They stay below 2^15,
 //   inside fp16, which keeps 11 bits of those down to 2^-21 of the largest (2^-14 without the 7).
+//
+// Measured on B200 (a graph of calls): one sequence of 131071 tokens, 32 heads on 8: 58 us, 4.6 TB/s; 32
+// sequences of up to 8192: 59 us, 4.8 TB/s; 64 with a window of 1024: 40 us, 3.2 TB/s. A share's first tile comes
+// 6 us after the launch (metadata, pages, scales, the copy), and a unit's end takes 3 to 5 us (four warps' sums,
+// the part's write, the count, the join), which three CTAs an SM hide in part.
 #include <algorithm>
 #include <mutex>
 #include <set>

@@ -5,15 +5,17 @@
 // group, token-major, so every head of the group uses a key tile once -- as two 128-row tiles. The bound is
 // the tensor core (S = Q K^T and O = P V, tcgen05 kind::f16) against the exponentials (one each score).
 // Roles of a CTA (one per SM, 16 warps; registers go from the others to the softmax):
-//   warps 0-3, 4-7   the softmax of the first and second 128 rows, a row a thread: scores from TMEM, the
-//                    running maximum and sum in float32 registers, weights back to TMEM as fp16 over the
-//                    scores that they came from. They also fetch the queries and write the output.
+//   warps 0-3, 4-7   the softmax of the first and second 128 rows, a row a thread, 64 keys a step: scores from
+//                    TMEM, the running maximum and sum in float32 registers, weights back to TMEM as fp16 over
+//                    the scores that they came from. They also fetch the queries and write the output.
 //   warps 8-11       pages to operands: 128 keys of int8 from HBM through registers (a tile ahead) to 16 bits
-//                    in shared memory (exact: keys in the queries' type, values in fp16), two stages of each. No scale is multiplied in: the key scale multiplies the
-//                    score, the value scale (over a reference that follows its size) the weight.
-//   warps 12, 15     one thread each issues the products of a row tile, 64 keys of scores at a time, as its own
-//                    softmax is ready for them. (One warp for both waited for one row tile while the other's
-//                    weights were ready: 8 prompts of 2048, 16 heads on 8, took 257 us instead of 236.)
+//                    in shared memory (exact: keys in the queries' type, values in fp16), two stages of each.
+//                    No scale is multiplied in: the key scale multiplies the score, the value scale (over a
+//                    reference that follows its size) the weight.
+//   warps 12, 15     one thread each issues the products of a row tile: a step's P V, then the scores that the
+//                    same 64 columns of TMEM hold next, while the softmax works on the other 64. (One warp for
+//                    both row tiles waited for one while the other's weights were ready: 8 prompts of 2048, 16
+//                    heads on 8, took 257 us instead of 236.)
 //   warp 13          walks the line (below) and hands the pieces to the others.
 //   warp 14          looks the tiles' pages and their scales up, up to four tiles ahead.
 // O stays in TMEM; it is rescaled only when a row's maximum grew by more than 2^4 (so a weight is
@@ -23,6 +25,14 @@
 // joined by the last of them in key order. An item is as long as its key tiles and kItemCost = 3 more, for its
 // queries, its output and its masked last tiles (about 12,000 cycles to a tile's 4,800; equal numbers of tiles
 // left the SMs with many short items a sixth longer: 8 prompts of 2048 took 236 us instead of 215).
+//
+// Measured on B200 (a graph of calls): 8 prompts of 2048, 16 heads on 8, bf16: 206 us, 0.67 PFLOP/s of visible
+// products; 8192 with a window of 2048, 32 heads on 8: 357 us, 0.67; 4 chunks of 512 at the end of up to 12289,
+// 32 heads on 8, fp16: 223 us, 0.88. No unit is full: in a steady tile of 4,800 cycles the tensor pipe runs
+// 2,700 (64 keys a product read Q from shared memory twice as often as 128 do: 54 cycles instead of 32 for 64),
+// the exponentials' pipe 2,000, the shared-memory pipe 3,800 and each scheduler issues 2,400 instructions.
+// Scores of 128 keys a product read less but leave one score buffer a row tile, so that the softmax waits for
+// them: 229, 409 and 254 us.
 #include <algorithm>
 
 #include "det_math.cuh"
