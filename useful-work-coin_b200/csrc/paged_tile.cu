@@ -22,13 +22,14 @@
 // below 1024 * 2^4 * 2 in fp16, and keeps its 11 bits down to 2^-24 of the reference) or the tile's largest value
 // scale left [1/64, 2] of the reference; both are rare after an item's first tile.
 // Items lie on one line, cut into equal parts, one per SM, as in the few-row form; an item in several parts is
-// joined by the last of them in key order. An item is as long as its key tiles and kItemCost = 3 more, for its
-// queries, its output and its masked last tiles (about 12,000 cycles to a tile's 4,800; equal numbers of tiles
-// left the SMs with many short items a sixth longer: 8 prompts of 2048 took 236 us instead of 215).
+// joined by the last of them in key order. An item is as long as its key tiles and kItemCost = 2 more, for its
+// queries, its output and its masked tiles: equal numbers of tiles left the SMs with many short items
+// longest (with 0, 1, 2 and 3 more: 8 prompts of 2048, 16 heads on 8, 204, 196, 195 and 199 us; 8192 tokens with a
+// window of 2048, 32 heads on 8, 361, 332, 313 and 315).
 //
-// Measured on B200 (a graph of calls): 8 prompts of 2048, 16 heads on 8, bf16: 204 us, 0.67 PFLOP/s of visible
-// products; 8192 with a window of 2048, 32 heads on 8: 338 us, 0.71; 4 chunks of 512 at the end of up to 12289,
-// 32 heads on 8, fp16: 224 us, 0.88. No unit is full: in a steady tile of 4,800 cycles the tensor pipe runs
+// Measured on B200 (a graph of calls): 8 prompts of 2048, 16 heads on 8, bf16: 195 us, 0.70 PFLOP/s of visible
+// products; 8192 with a window of 2048, 32 heads on 8: 313 us, 0.77; 4 chunks of 512 at the end of up to 12289,
+// 32 heads on 8, fp16: 225 us, 0.88. No unit is full: in a steady tile of 4,800 cycles the tensor pipe runs
 // 2,700 (64 keys a product read Q from shared memory twice as often as 128 do: 54 cycles instead of 32 for 64),
 // the exponentials' pipe 2,000, the shared-memory pipe 3,800 and each scheduler issues 2,400 instructions.
 // Scores of 128 keys a product read less but leave one score buffer a row tile, so that the softmax waits for
@@ -54,7 +55,7 @@ constexpr int kPageRing = 8;                 // slots: those, and up to four tha
 constexpr int kSeqs = 1024;                  // sequences whose span and tiles are kept in shared memory
 constexpr int kSmem = 1024 + 6 * kOperand + kSeqs * 24;   // two query tiles, two stages of keys, two of values
 constexpr int kMinTiles = 4;                 // a CTA's least share of the line
-constexpr int kItemCost = 3;                 // what an item costs beside its tiles, in tiles
+constexpr int kItemCost = 2;                 // what an item costs beside its tiles, in tiles
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 // 128 dims; values are stored key by key: B is MN-major
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(kHd >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
