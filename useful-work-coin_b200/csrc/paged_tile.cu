@@ -4,7 +4,8 @@
 // k_paged_tile: an item is 256 rows of one (sequence, KV head) -- its tokens times the query heads of the
 // group, token-major, so every head of the group uses a key tile once -- as two 128-row tiles. The bound is
 // the tensor core (S = Q K^T and O = P V, tcgen05 kind::f16) against the exponentials (one each score).
-// Roles of a CTA (one per SM, 16 warps; registers go from the others to the softmax):
+// Roles of a CTA (one per SM, 16 warps; registers go from the others to the softmax: with 144 and 112 the third
+// case below takes 221 us, with 152 and 96 or 112 225, with 128 for all, and spills, 224):
 //   warps 0-3, 4-7   the softmax of the first and second 128 rows, a row a thread, 64 keys a step: scores from
 //                    TMEM, the running maximum and sum in float32 registers, weights back to TMEM as fp16 over
 //                    the scores that they came from. They also fetch the queries and write the output.
@@ -27,9 +28,9 @@
 // longest (with 0, 1, 2 and 3 more: 8 prompts of 2048, 16 heads on 8, 204, 196, 195 and 199 us; 8192 tokens with a
 // window of 2048, 32 heads on 8, 361, 332, 313 and 315).
 //
-// Measured on B200 (a graph of calls): 8 prompts of 2048, 16 heads on 8, bf16: 195 us, 0.70 PFLOP/s of visible
-// products; 8192 with a window of 2048, 32 heads on 8: 313 us, 0.77; 4 chunks of 512 at the end of up to 12289,
-// 32 heads on 8, fp16: 225 us, 0.88. No unit is full: in a steady tile of 4,800 cycles the tensor pipe runs
+// Measured on B200 (a graph of calls): 8 prompts of 2048, 16 heads on 8, bf16: 195 us, 0.71 PFLOP/s of visible
+// products; 8192 with a window of 2048, 32 heads on 8: 312 us, 0.77; 4 chunks of 512 at the end of up to 12289,
+// 32 heads on 8, fp16: 221 us, 0.89. No unit is full: in a steady tile of 4,800 cycles the tensor pipe runs
 // 2,700 (64 keys a product read Q from shared memory twice as often as 128 do: 54 cycles instead of 32 for 64),
 // the exponentials' pipe 2,000, the shared-memory pipe 3,800 and each scheduler issues 2,400 instructions.
 // Scores of 128 keys a product read less but leave one score buffer a row tile, so that the softmax waits for
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   const int Hkv = a.c.Hkv, ps = a.c.ps, G = a.H / Hkv;
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // ------------------------------------------------------------------ softmax, a row a thread
     const int w = warp >> 2, r = tid & (kRows - 1);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -651,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       TILE_PIECE_DONE(n);
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     // ------------------------------------------------------------------ pages to operands
     // A thread: key row % 16 and 16 dims from 16 c on. Eight lanes have the eight c of two neighbouring rows, four
     // of each: neither their loads (a bank each) nor, swizzled into the two blocks, their stores conflict.
