@@ -187,7 +187,8 @@ class PagedBatch:
     def verify(self, drafts: dict[int, list[int]]) -> dict[int, list[int]]:
         """One step for the slots of `drafts`, with tokens guessed to follow each one's newest: the greedy tokens
         that the model itself puts there, up to and with the first that differs from the guess. The cache keeps
-        what was confirmed; a rejected token's place is written again by the next call."""
+        what was confirmed; a rejected token's place is written again by the next call (its page's scale stays as it
+        grew, if it did)."""
         if not drafts:
             return {}
         slots = sorted(drafts)
