@@ -178,18 +178,26 @@ def quant_rows_had(x: torch.Tensor, bs: int, q: torch.Tensor | None = None, scal
     return q, scale
 
 
-def gemm_workspace(device, m: int, n: int, flags: int, out_mode: int) -> torch.Tensor | None:
-    """Per-device workspace of the hashed GEMM (tile messages; the int32 product of a denoised bf16
-    forward), grown on demand. Callers serialize on one stream per device (like the reference's
-    shared workspace, ops.py:258-277)."""
-    nbytes = int(lib().uwc_gemm_workspace_bytes(m, n, flags, out_mode))
+def _gemm_scratch(device, nbytes: int) -> torch.Tensor | None:
+    """A GEMM call's scratch: the device's buffer, grown on demand, and in a capture one of the graph's own
+    pool. (A graph replays on the address that it was captured with; the device's buffer is freed when a later
+    call of more rows replaces it.)"""
     if nbytes == 0:
         return None
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = str(torch.device(device))
     ws = _GEMM_WS.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = _GEMM_WS[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return ws
+
+
+def gemm_workspace(device, m: int, n: int, flags: int, out_mode: int) -> torch.Tensor | None:
+    """Per-device workspace of the hashed GEMM (tile messages; the int32 product of a denoised bf16
+    forward), grown on demand. Callers serialize on one stream per device (like the reference's
+    shared workspace, ops.py:258-277)."""
+    return _gemm_scratch(device, int(lib().uwc_gemm_workspace_bytes(m, n, flags, out_mode)))
 
 
 def gemm(A, B, *, r=128, flags=0, corrA=None, corrB=None, maxabs=None, key=None, target=None, wins=None,
@@ -244,13 +252,7 @@ def gemm_epi(X, W, epi=SEPI_I32, *, x_scale=None, w_scale=None, resid=None, out=
         out = torch.empty((m, n // 2 if epi == SEPI_SWIGLU else n), dtype=dt, device=X.device)
     f32 = (lambda t: None if t is None else t.contiguous().float())
     flags = epi | (SEPI_EARLY_W if early_w else 0)
-    nbytes = int(lib().uwc_gemm_epi_workspace_bytes(m, n, epi))
-    ws = None
-    if nbytes:
-        key = str(torch.device(X.device))
-        ws = _GEMM_WS.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = _GEMM_WS[key] = torch.empty(nbytes, dtype=torch.uint8, device=X.device)
+    ws = _gemm_scratch(X.device, int(lib().uwc_gemm_epi_workspace_bytes(m, n, epi)))
     check(lib().uwc_gemm_epi(_p(X), _p(W), m, n, k, _p(f32(x_scale)), _p(f32(w_scale)),
                              _p(None if resid is None else resid.contiguous()), _p(out), flags, _p(ws),
                              0 if ws is None else ws.numel(), _stream()), "gemm_epi")
