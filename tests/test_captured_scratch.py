@@ -69,3 +69,34 @@ def test_a_batch_of_many_slots_keeps_its_scratch(dev, monkeypatch):
     for x in (b, eager):
         x.said = [x.admit(prompts[:1]), x.step(), x.admit(prompts[1:]), x.step(), x.step()]
     assert b.said == eager.said
+
+
+def allocated(p):
+    """Whether torch's allocator holds the address for some tensor."""
+    for s in torch.cuda.memory_snapshot():
+        at = s["address"]
+        for x in s["blocks"]:
+            if at <= p < at + x["size"]:
+                return x["state"] == "active_allocated"
+            at += x["size"]
+    return False
+
+
+@pytest.mark.gpu
+def test_a_graphed_forward_keeps_its_workspace(dev, monkeypatch):
+    """The weights of a device share a workspace; a graph's outlives its replacement by a larger one."""
+    from uwc_b200 import ops
+    monkeypatch.setattr(ops, "_SHARED_WS", {})
+    m, n, k = 256, 512, 2048
+    g = torch.Generator(device=dev).manual_seed(3)
+    i8 = lambda *s: torch.randint(-64, 65, s, device=dev, generator=g, dtype=torch.int8)
+    A = i8(m, k)
+    w = ops.MinedWeight(Bt=i8(n, k), b_scale=torch.ones(n, device=dev))
+    w.setup_block(bytes(range(32)), [0] * 8)
+    gf = ops.GraphedForward(w, m, out_mode=ops.OUT_I32)
+    p = w._last_ws[m][0].data_ptr()
+    ops.shared_workspace(dev, 2 * w._last_ws[m][0].numel())
+    want = w.forward(A, gf.a_scale, out_mode=ops.OUT_I32)        # on the larger one
+    assert w._last_ws[m][0].data_ptr() != p and allocated(p)
+    gf.A.copy_(A)
+    assert torch.equal(gf(), want)

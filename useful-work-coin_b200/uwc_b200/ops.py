@@ -454,6 +454,7 @@ class GraphedForward:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             call()
+        self.workspace = w._last_ws[m][0]   # the graph's, also after the weights' shared one was replaced by a larger
 
     def __call__(self) -> torch.Tensor:
         self.graph.replay()
