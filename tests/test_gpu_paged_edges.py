@@ -1,0 +1,40 @@
+"""The paged operators at the edges of their arguments: integers far outside an int, tensors without a row, batches
+without a sequence, queries and keys at the ends of bf16's range, integers of -128 in a caller's pages."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from paged_fixture import D, Batch, append_plain, random_cache
+from test_gpu_paged import BF, HF, fused_rows, numpy_cache, status_clean, tables  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("most", [1, 8, 60])
+@pytest.mark.parametrize("cu", [(5, -2 ** 31), (1, 2 - 2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1 - 60),
+                                (-2 ** 31, 2 ** 31 - 1), (-2 ** 31, -2 ** 31)], ids=str)
+def test_row_offsets_at_the_ends_of_int(dev, cu, most):
+    """Row offsets that are no rows: those of the tensors that they name (rows 0 and on, for a lower end below 0) may
+    be written, none else, and the status says so."""
+    from uwc_b200 import _lib, paged
+    b = Batch([100], [1], 16)
+    cache = random_cache(b, 2, dev)
+    before = {n: t.clone() for n, t in cache.items()}
+    table, _, _ = b.device(dev)
+    start = torch.tensor([10], dtype=torch.int32, device=dev)
+    c = torch.tensor(cu, dtype=torch.int32, device=dev)
+    _, _, cosd, sind = tables(128, dev)
+    q, k, v = fused_rows(7, 4, 2, BF, dev, 0)
+    out = torch.full((7, 4, D), 7.0, dtype=BF, device=dev)
+    named = cu[0] < 0 and cu[1] > 0
+    paged.attention(q, cache, table, start, c, most, 100, out=out)
+    assert _lib.device_status(clear=True) == _lib.DEV_RANGE
+    assert (out[min(most, 7) if named else 0:] == 7.0).all()
+    paged.append(k, v, cache, table, start, c, most, cosd, sind, q=q)
+    assert _lib.device_status(clear=True) == _lib.DEV_RANGE
+    if not named:
+        assert all(torch.equal(before[n], cache[n]) for n in cache)
+    paged.gather(cache, table, start, c, 7, most)
+    assert _lib.device_status(clear=True) == _lib.DEV_RANGE

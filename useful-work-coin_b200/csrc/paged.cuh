@@ -46,8 +46,8 @@ __device__ __forceinline__ Span span_of(const Seqs& b, int ps, int s) {
   r.start = __ldg(b.start + s);
   r.row0 = max(c0, 0);
   r.idle = r.start < 0;
-  const int hi = min(c1, b.rows);
-  r.n = min(max(hi - r.row0, 0), b.max_new);
+  const int hi = max(min(c1, b.rows), r.row0);     // no difference below overflows, whatever the two hold
+  r.n = min(hi - r.row0, b.max_new);
   if (!r.idle) r.n = max(0, min(r.n, b.width * ps - r.start));   // width * ps < 2^31: the host checks
   r.bad = c0 < 0 || c1 < c0 || r.n != c1 - c0;
   return r;
