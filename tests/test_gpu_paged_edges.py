@@ -12,6 +12,29 @@ from test_gpu_paged import BF, HF, fused_rows, numpy_cache, status_clean, tables
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("value", [-1, -2 ** 31, -2 ** 32, 5 - 2 ** 32, -2 ** 63])
+def test_negative_windows_and_sinks_are_refused(dev, value):
+    from uwc_b200 import paged
+    b = Batch([40], [1], 16)
+    cache = random_cache(b, 1, dev)
+    q, _, _ = fused_rows(1, 2, 1, BF, dev, 0)
+    with pytest.raises(AssertionError):
+        paged.attention(q, cache, *b.device(dev), 1, 40, window=value)
+    with pytest.raises(AssertionError):
+        paged.attention(q, cache, *b.device(dev), 1, 40, window=8, sinks=value)
+
+
+@pytest.mark.parametrize("value", [2 ** 31, 2 ** 40, 2 ** 63 - 1])
+def test_windows_past_every_position_are_none(dev, value):
+    from uwc_b200 import paged
+    b = Batch([40], [1], 16)
+    cache = random_cache(b, 1, dev)
+    q, _, _ = fused_rows(1, 2, 1, BF, dev, 0)
+    want = paged.attention(q, cache, *b.device(dev), 1, 40)
+    assert torch.equal(paged.attention(q, cache, *b.device(dev), 1, 40, window=value), want)
+    assert torch.equal(paged.attention(q, cache, *b.device(dev), 1, 40, window=3, sinks=value), want)
+
+
 @pytest.mark.parametrize("most", [1, 8, 60])
 @pytest.mark.parametrize("cu", [(5, -2 ** 31), (1, 2 - 2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1 - 60),
                                 (-2 ** 31, 2 ** 31 - 1), (-2 ** 31, -2 ** 31)], ids=str)

@@ -42,6 +42,12 @@ int length(PyObject* o, const char* what) {
   require(v >= 0 && v <= kMost, what);
   return (int)v;
 }
+// A window or a number of sinks: more than any position is as good as kMost.
+int reach(PyObject* o, const char* what) {
+  const long long v = integer(o);
+  require(v >= 0, what);
+  return (int)std::min(v, kMost);
+}
 double real(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw std::bad_cast();
@@ -233,10 +239,8 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int code = type_code(type);
     const Rows q = rows_of(c, qt, type);
     const double scale = real(a[10]);
-    const int window = a[11] == Py_None ? -1 : (int)std::min(integer(a[11]), kMost);
-    require(a[11] == Py_None || window >= 0, "window is not negative");
-    const int sinks = (int)std::min(integer(a[12]), kMost);
-    require(sinks >= 0, "sinks is not negative");
+    const int window = a[11] == Py_None ? -1 : reach(a[11], "window is not negative");
+    const int sinks = reach(a[12], "sinks is not negative");
     at::Tensor out;
     if (a[13] == Py_None) {
       out = at::empty({q.n, q.heads, kHd}, qt.options());
