@@ -447,7 +447,8 @@ int uwc_stage_roots(const float* rows, int B, int T, int D, uint32_t* scratch, u
  * max_len >= every start[s] + new tokens (attention; sizes the split, exceeding it is safe but slow).
  * Metadata out of its range (a page outside the pool, a position past the table or the rotation
  * table, rows past `rows`, more than max_new new tokens) is skipped and raises UWC_DEV_RANGE in
- * uwc_device_status. Rows that no sequence covers are not written. A page may be shared by several
+ * uwc_device_status. Rows that no sequence covers are not written. With rows == 0 the row tensors, and with
+ * seqs == 0 the batch's description, may be NULL: nothing is done. A page may be shared by several
  * tables (a common prefix) as long as no call appends to it from more than one.
  * dtype: UWC_T_BF16 or UWC_T_F16, of every row tensor of the call. Row tensors may be strided: element
  * (n, h, d) at n * tok + h * head + d; strides are multiples of 8 elements, base pointers 16-byte aligned. */

@@ -35,6 +35,31 @@ def test_windows_past_every_position_are_none(dev, value):
     assert torch.equal(paged.attention(q, cache, *b.device(dev), 1, 40, window=3, sinks=value), want)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_no_rows_and_no_sequences(dev, dtype):
+    """Nothing to do is done: tensors of no row, which have no address, and a batch of no sequence."""
+    from uwc_b200 import paged
+    b = Batch([40, 9], [0, 0], 16)
+    cache = random_cache(b, 2, dev)
+    before = {n: t.clone() for n, t in cache.items()}
+    table, start, cu = b.device(dev)
+    _, _, cosd, sind = tables(64, dev)
+    q, k, v = fused_rows(0, 4, 2, dtype, dev, 0)
+    none = torch.empty(0, b.width, dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev), cu[:1]
+    for t, s, c in ((table, start, cu), none):
+        assert paged.append(k, v, cache, t, s, c, 0, cosd, sind) is None
+        assert paged.append(k, v, cache, t, s, c, 3, cosd, sind, q=q).shape == (0, 4, D)
+        assert paged.attention(q, cache, t, s, c, 0, 40).shape == (0, 4, D)
+        x, y = paged.gather(cache, t, s, c, 0, 0, dtype=dtype)
+        assert x.shape == y.shape == (0, 2, D) and x.dtype == dtype
+    # rows that no sequence covers stay as they are
+    q, k, v = fused_rows(3, 4, 2, dtype, dev, 0)
+    out = torch.full((3, 4, D), 7.0, dtype=dtype, device=dev)
+    paged.attention(q, cache, *none, 1, 40, out=out)
+    paged.append(k, v, cache, *none, 1, cosd, sind)
+    assert (out == 7.0).all() and all(torch.equal(before[n], cache[n]) for n in cache)
+
+
 @pytest.mark.parametrize("most", [1, 8, 60])
 @pytest.mark.parametrize("cu", [(5, -2 ** 31), (1, 2 - 2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1 - 60),
                                 (-2 ** 31, 2 ** 31 - 1), (-2 ** 31, -2 ** 31)], ids=str)

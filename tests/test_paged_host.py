@@ -85,3 +85,16 @@ def test_python_refusals():
         paged.gather(cache, z(1, 4), z(1), z(2), 1, 1)
     with pytest.raises(AssertionError):
         paged.append(q[:, :2], q[:, :2], cache, z(1, 4), z(1), z(2), 1, None, None)
+
+
+@pytest.mark.parametrize("none", [dict(rows=0), dict(seqs=0)], ids=str)
+def test_nothing_to_do_needs_no_address(none):
+    """Row tensors of no row and descriptions of no sequence have none: the call passes its checks and gets as far as
+    the device's."""
+    from uwc_b200 import _lib
+    names = {"rows": ("k", "v", "q", "q_out", "out"), "seqs": ("table", "start", "first", "cu")}[next(iter(none))]
+    for f, base in (("append", base_append), ("attention", base_attention), ("gather", base_gather)):
+        a = base()
+        a.update(none, **{n: None for n in names if n in a})
+        rc = getattr(_lib.lib(), f"uwc_paged_{f}")(*a.values())
+        assert rc in (_lib.OK, _lib.ERR_CUDA, _lib.ERR_DEVICE), (f, rc)

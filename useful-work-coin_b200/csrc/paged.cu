@@ -528,7 +528,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 int uwc_paged_check(Cache* cache, const Seqs* seqs) {
   Cache& c = *cache;
   const Seqs& b = *seqs;
-  if (!c.k || !c.sk || !c.v || !c.sv || !b.table || !b.start || !b.cu) return UWC_ERR_ARG;
+  if (!c.k || !c.sk || !c.v || !c.sv || (b.seqs && (!b.table || !b.start || !b.cu))) return UWC_ERR_ARG;
   if (c.pages < 1 || c.Hkv < 1 || (c.ps != 16 && c.ps != 32 && c.ps != 64 && c.ps != 128)) return UWC_ERR_SHAPE;
   if (b.seqs < 0 || b.seqs > 65535 || b.width < 1 || b.rows < 0 || b.max_new < 0) return UWC_ERR_SHAPE;
   if ((long long)b.width * c.ps > (1ll << 30) || b.rows > (1 << 30)) return UWC_ERR_SHAPE;
@@ -583,7 +583,7 @@ extern "C" int uwc_paged_append(int8_t* kc, float* sk, int8_t* vc, float* sv, in
   a.b = Seqs{table, start, cu, seqs, width, rows, max_new};
   const int rc = uwc_paged_check(&a.c, &a.b);
   if (rc != UWC_OK) return rc;
-  if (!k || !v || !cos || !sin || (dtype != UWC_T_BF16 && dtype != UWC_T_F16) || (q && !q_out)) return UWC_ERR_ARG;
+  if ((rows && (!k || !v)) || !cos || !sin || (dtype != UWC_T_BF16 && dtype != UWC_T_F16) || (q && !q_out)) return UWC_ERR_ARG;
   if (max_pos < 1 || (q && H < 1)) return UWC_ERR_SHAPE;
   if (!aligned16(k) || !aligned16(v) || !aligned16(cos) || !aligned16(sin) || !row_strides_ok(k_tok, k_head) ||
       !row_strides_ok(v_tok, v_head))
@@ -619,7 +619,7 @@ extern "C" int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t*
   a.b = Seqs{table, first, cu, seqs, width, rows, max_rows};
   const int rc = uwc_paged_check(&a.c, &a.b);
   if (rc != UWC_OK) return rc;
-  if (!k || !v || (dtype != UWC_T_BF16 && dtype != UWC_T_F16 && dtype != UWC_T_F32)) return UWC_ERR_ARG;
+  if ((rows && (!k || !v)) || (dtype != UWC_T_BF16 && dtype != UWC_T_F16 && dtype != UWC_T_F32)) return UWC_ERR_ARG;
   if (!aligned16(k) || !aligned16(v)) return UWC_ERR_ALIGN;
   UWC_CHECK_DEVICE();
   if (seqs == 0 || rows == 0 || max_rows == 0) return UWC_OK;

@@ -178,7 +178,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                            q.heads, (const float*)cos.data_ptr(), (const float*)sin.data_ptr(), (int)cos.size(0), norm[0],
                            norm[1], eps, c10::cuda::getCurrentCUDAStream(c.dev).stream()),
           "paged append");
-    if (!q.p) Py_RETURN_NONE;
+    if (a[12] == Py_None) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   });
 }
