@@ -477,7 +477,7 @@ int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t* vc, const 
 /* Attention of the new tokens over their sequence's pages, which already hold them: the query at
  * position p sees key j when j <= p and (window < 0, or j > p - window, or j < sinks). q (rows, H, 128),
  * H a multiple of Hkv (head h reads KV head h / (H / Hkv)); out (rows, H, 128) contiguous, in dtype.
- * softmax(scale q . k) in float32; a row that sees no key is zero. No atomics touch a result: the same
+ * softmax(scale q . k) in float32, scale finite; a row that sees no key is zero. No atomics touch a result: the same
  * call gives the same bits. workspace: uwc_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
  * whose first 4096 are zero before its first use (counters; every call leaves them zero). Calls that
  * overlap on the GPU must not share one. */

@@ -60,6 +60,16 @@ def test_no_rows_and_no_sequences(dev, dtype):
     assert (out == 7.0).all() and all(torch.equal(before[n], cache[n]) for n in cache)
 
 
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_a_scale_that_is_not_finite_is_refused(dev, scale):
+    from uwc_b200 import paged
+    for new in (1, 40):
+        b = Batch([40], [new], 16)
+        q, _, _ = fused_rows(new, 2, 1, BF, dev, 0)
+        with pytest.raises(AssertionError):
+            paged.attention(q, random_cache(b, 1, dev), *b.device(dev), new, 40, scale=scale)
+
+
 @pytest.mark.parametrize("most", [1, 8, 60])
 @pytest.mark.parametrize("cu", [(5, -2 ** 31), (1, 2 - 2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1 - 60),
                                 (-2 ** 31, 2 ** 31 - 1), (-2 ** 31, -2 ** 31)], ids=str)

@@ -98,3 +98,9 @@ def test_nothing_to_do_needs_no_address(none):
         a.update(none, **{n: None for n in names if n in a})
         rc = getattr(_lib.lib(), f"uwc_paged_{f}")(*a.values())
         assert rc in (_lib.OK, _lib.ERR_CUDA, _lib.ERR_DEVICE), (f, rc)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_attention_refuses_a_scale_that_is_not_finite(scale):
+    from uwc_b200 import _lib
+    assert _lib.lib().uwc_paged_attention(*{**base_attention(), "scale": scale}.values()) == _lib.ERR_ARG

@@ -30,6 +30,7 @@
 // 6 us after the launch (metadata, pages, scales, the copy), and a unit's end takes 3 to 5 us (four warps' sums,
 // the part's write, the count, the join), which three CTAs an SM hide in part.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -705,6 +706,7 @@ extern "C" int uwc_paged_attention(const int8_t* kc, const float* sk, const int8
   const int rc = uwc_paged_check(&a.c, &a.b);
   if (rc != UWC_OK) return rc;
   if ((rows && (!q || !out)) || (dtype != UWC_T_BF16 && dtype != UWC_T_F16)) return UWC_ERR_ARG;
+  if (!std::isfinite(scale)) return UWC_ERR_ARG;
   if (H < 1 || H % Hkv || max_len < 0 || sinks < 0) return UWC_ERR_SHAPE;
   if ((long long)max_new * (H / Hkv) > (1ll << 30)) return UWC_ERR_SHAPE;   // a sequence's rows are counted in int
   if (((uintptr_t)q | (uintptr_t)out) & 15 || q_tok < 0 || q_head < 0 || q_tok % 8 || q_head % 8) return UWC_ERR_ALIGN;
