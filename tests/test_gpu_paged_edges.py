@@ -96,3 +96,24 @@ def test_row_offsets_at_the_ends_of_int(dev, cu, most):
         assert all(torch.equal(before[n], cache[n]) for n in cache)
     paged.gather(cache, table, start, c, 7, most)
     assert _lib.device_status(clear=True) == _lib.DEV_RANGE
+
+
+@pytest.mark.parametrize("max_new", [70, 2 ** 30, 2 ** 31 - 126, 2 ** 31 - 1])
+def test_append_with_any_bound_on_new_tokens(dev, max_new):
+    """The bound may be as loose as an int is wide (the C entry's; uwc_b200.paged takes it up to 2^30)."""
+    from uwc_b200 import _lib, paged
+    for ps in (16, 128):
+        b = Batch([100, 3], [70, 2], ps)
+        cache = random_cache(b, 2, dev)
+        want = {n: t.clone() for n, t in cache.items()}
+        table, start, cu = b.device(dev)
+        _, _, cosd, sind = tables(128, dev)
+        q, k, v = (t.contiguous() for t in fused_rows(72, 4, 2, BF, dev, 0))
+        rot = paged.append(k, v, want, table, start, cu, 70, cosd, sind, q=q)
+        got = torch.empty_like(q)
+        a = lambda t: t.data_ptr()
+        args = [a(cache["k"]), a(cache["sk"]), a(cache["v"]), a(cache["sv"]), b.pages, ps, 2, a(table), a(start), a(cu), 2,
+                b.width, 72, max_new, 0, a(k), 2 * D, D, a(v), 2 * D, D, a(q), 4 * D, D, a(got), 4, a(cosd), a(sind), 128,
+                None, None, 1e-6, torch.cuda.current_stream().cuda_stream]
+        assert _lib.lib().uwc_paged_append(*args) == _lib.OK
+        assert torch.equal(got, rot) and all(torch.equal(cache[n], want[n]) for n in cache)

@@ -13,6 +13,7 @@
 // Both are bound by HBM at prompt sizes and by latency at decode sizes. Measured on B200 (a graph of calls): 8
 // prompts of 2048, 16 + 2 x 8 heads, 63 us (3.7 TB/s: about 20 instructions a value, twice over the rows) and 20 us
 // to read it back; a token each of 64 sequences, 32 + 2 x 8 heads, 4.8 us.
+#include <algorithm>
 #include <cfloat>
 
 #include "det_math.cuh"
@@ -597,7 +598,7 @@ extern "C" int uwc_paged_append(int8_t* kc, float* sk, int8_t* vc, float* sv, in
   a.q_out = q_out;
   a.H = H;
   a.max_pos = max_pos;
-  a.most = min((max_new + page_size - 2) / page_size + 1, width);
+  a.most = (int)std::min(((long long)max_new + page_size - 2) / page_size + 1, (long long)width);
   a.cos = cos;
   a.sin = sin;
   a.q_norm = q_norm;
