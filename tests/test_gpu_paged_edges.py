@@ -70,6 +70,21 @@ def test_a_scale_that_is_not_finite_is_refused(dev, scale):
             paged.attention(q, random_cache(b, 1, dev), *b.device(dev), new, 40, scale=scale)
 
 
+@pytest.mark.parametrize("e", [100, 116, 125, 127])
+def test_queries_up_to_the_largest(dev, e):
+    """Single tokens whose largest query value is near 2^e, on keys as much smaller: the scores are ordinary."""
+    from test_gpu_paged_scales import check_rows
+    b = Batch([300, 17], [1, 1], 64, seed=e)
+    cache = random_cache(b, 2, dev, e, spread=0.3)
+    q, _, _ = fused_rows(2, 4, 2, BF, dev, e)
+    up = math.ldexp(1.0, e - 2)                            # the rows' largest are below 4
+    assert float(q.abs().max()) < 4
+    cache["sk"] *= 2.0 ** -60
+    plain = {**cache, "sk": cache["sk"] * 2.0 ** 60}
+    check_rows(dev, b, plain, q)
+    check_rows(dev, b, cache, (q.double() * up).to(BF), scale=math.ldexp(1 / math.sqrt(D), 62 - e))
+
+
 @pytest.mark.parametrize("most", [1, 8, 60])
 @pytest.mark.parametrize("cu", [(5, -2 ** 31), (1, 2 - 2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1 - 60),
                                 (-2 ** 31, 2 ** 31 - 1), (-2 ** 31, -2 ** 31)], ids=str)

@@ -128,10 +128,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// The exponent e that brings a row whose largest magnitude is mx to [2^14, 2^15): q 2^e is its fp16 form.
+// The exponent e that brings a row whose largest magnitude is mx to [2^14, 2^15) (up to 2^127, down to 2^-86; what is
+// smaller still stays below that): q 2^e is its fp16 form.
 __device__ __forceinline__ int row_exponent(float mx) {
   const int x = (__float_as_int(mx) >> 23) & 255;
-  return mx == 0.f || x == 255 ? 0 : min(max(14 + 127 - x, -100), 100);
+  return mx == 0.f || x == 255 ? 0 : min(14 + 127 - x, 100);
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
