@@ -43,3 +43,52 @@ def setup(dev, lens, new, ps, Hkv, dtype, seed, amp=1.0):
     cache = random_cache(b, Hkv, dev, seed, spread=0.0)
     q, _, _ = fused_rows(b.rows, 2 * Hkv, Hkv, dtype, dev, seed, amp)
     return b, cache, q
+
+
+@pytest.mark.parametrize("new", FORMS)
+@pytest.mark.parametrize("small", [0.0, 1e-39, 1e-38, 1e-36, 1e-33, 1e-31, 1e-20])
+def test_value_scales_of_almost_nothing(dev, small, new):
+    """A head whose values are (almost) nothing, in all pages, in the first ones or in the last ones."""
+    for where in (slice(0, None), slice(0, 4), slice(4, None), slice(6, 7)):
+        b, cache, q = setup(dev, [140, 137], [new, new], 16, 2, BF, 3)
+        for s in range(2):
+            pages = b.table[s][:9].tolist()[where]
+            cache["sv"][pages, s] = small
+        check_rows(dev, b, cache, q)
+        check_rows(dev, b, cache, q, window=50, sinks=3)
+
+
+@pytest.mark.parametrize("small", [1e-4, 1e-6, 1e-9, 1e-12])
+def test_rows_do_not_lose_bits_to_pages_that_they_do_not_see(dev, small):
+    """A prompt whose first page's values are far smaller than the next ones': its first rows see no others."""
+    b, cache, q = setup(dev, [100, 300], [100, 250], 16, 2, BF, 5)
+    for s in range(2):
+        cache["sv"][b.table[s][0].item()] *= small
+        cache["sv"][b.table[s][3].item()] *= small
+    check_rows(dev, b, cache, q)
+    check_rows(dev, b, cache, q, window=16)
+
+
+def test_chunks_of_a_prompt_give_its_rows(dev):
+    """The first rows alone and as part of the prompt: the same within the rounding of their own values."""
+    from uwc_b200 import paged
+    b, cache, q = setup(dev, [120], [120], 16, 1, BF, 6)
+    cache["sv"][b.table[0][0].item()] *= 1e-9
+    all_rows = check_rows(dev, b, cache, q)
+    table, start, _ = b.device(dev)
+    head = paged.attention(q[:16], cache, table, start, torch.tensor([0, 16], dtype=torch.int32, device=dev), 16, 16)
+    o, absv, _ = attention64(q, cache, b, 1 / math.sqrt(D), None, 0)
+    off = (head.double() - all_rows[:16].double()).abs()
+    assert bool((off <= 2.0 ** -8 * o[:16].abs() + 2.0 ** -9 * absv[:16]).all())
+
+
+@pytest.mark.parametrize("new", FORMS)
+@pytest.mark.parametrize("decades", [6, 12, 20])
+def test_unlikely_keys_with_large_values(dev, decades, new):
+    """Scores of up to some 60 (in log2) and value scales over many decades: what decides a row's output may be keys
+    of next to no probability."""
+    for seed in range(4):
+        b, cache, q = setup(dev, [333, 90], [new, new], 16, 2, BF, seed, amp=2.0)
+        g = torch.Generator(device=dev).manual_seed(seed)
+        cache["sv"] = 10.0 ** (decades * (torch.rand(cache["sv"].shape, device=dev, generator=g) - 0.5))
+        check_rows(dev, b, cache, q)

@@ -11,17 +11,19 @@
 //                    the scores that they came from. They also fetch the queries and write the output.
 //   warps 8-11       pages to operands: 128 keys of int8 from HBM through registers (a tile ahead) to 16 bits
 //                    in shared memory (exact: keys in the queries' type, values in fp16), two stages of each.
-//                    No scale is multiplied in: the key scale multiplies the score, the value scale (over a
-//                    reference that follows its size) the weight.
+//                    No scale is multiplied in: the key scale multiplies the score, the value scale the weight.
 //   warps 12, 15     one thread each issues the products of a row tile: a step's P V, then the scores that the
 //                    same 64 columns of TMEM hold next, while the softmax works on the other 64. (One warp for
 //                    both row tiles waited for one while the other's weights were ready: 8 prompts of 2048, 16
 //                    heads on 8, took 257 us instead of 236.)
 //   warp 13          walks the line (below) and hands the pieces to the others.
 //   warp 14          looks the tiles' pages and their scales up, up to four tiles ahead.
-// O stays in TMEM; it is rescaled only when a row's maximum grew by more than 2^4 (so a weight is
-// below 1024 * 2^4 * 2 in fp16, and keeps its 11 bits down to 2^-24 of the reference) or the tile's largest value
-// scale left [1/64, 2] of the reference; both are rare after an item's first tile.
+// O stays in TMEM, in units of the row's own largest contribution: with m the running maximum of its scores (log2)
+// and v that of score + log2 s_v, over the keys that the row itself sees, a key's weight is 2^(score - m) s_v
+// 2^(m - v + 10). O is rescaled only when m or v grew by more than 4, which is rare after an item's first tile; so
+// weights stay below 2^14 in fp16 and keep 11 bits down to 2^-24 of the largest contribution, whatever lies in pages
+// that the mask hides from the row and however far apart the pages' scales are. (With one reference a tile, its largest
+// value scale, rows lost bits to later pages, and values below 4e-34 became NaN.)
 // Items lie on one line, cut into equal parts, one per SM, as in the few-row form; an item in several parts is
 // joined by the last of them in key order. An item is as long as its key tiles and kItemCost = 2 more, for its
 // queries, its output and its masked tiles: equal numbers of tiles left the SMs with many short items
@@ -36,6 +38,7 @@
 // Scores of 128 keys a product read less but leave one score buffer a row tile, so that the softmax waits for
 // them: 229, 409 and 254 us.
 #include <algorithm>
+#include <cfloat>
 
 #include "det_math.cuh"
 #include "paged.cuh"
@@ -61,7 +64,8 @@ constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_
 // 128 dims; values are stored key by key: B is MN-major
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(kHd >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 constexpr float kRaise = 4.f;                // log2 by which a score may pass the running maximum
-constexpr float kWeightUnit = 1024.f;         // the fp16 weight of p = 1 at the reference scale
+constexpr float kUnit = 10.f;                // log2 of the largest contribution's fp16 weight when v was set
+constexpr float kLow = 116.f;                // v is no lower than m by more: 2^(m - v + kUnit) is finite, 2^(v - m - kUnit) not 0
 
 struct TileArgs {
   AttnArgs a;
@@ -249,12 +253,6 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return r;
 }
 
-// What the softmax needs of a tile's pages: the largest value scale, and its 16-key groups that nobody sees.
-struct TileInfo {
-  float vmax;
-  int unseen;
-};
-
 struct Bars {
   uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], o_done[2][2], wg[2], piece_full[kPieces], piece_empty[kPieces], page_full[kAhead], page_empty[kAhead], fin;
 };
@@ -313,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   __shared__ Bars bar;
   __shared__ Piece s_piece[kPieces];
   __shared__ __align__(16) float2 s_scale[kPageRing][kGroups];   // factor of scores (log2), value scale
-  __shared__ TileInfo s_tile[kPageRing];
+  __shared__ __align__(16) float s_log[kPageRing][kGroups];      // log2 of the value scale
+  __shared__ int s_unseen[kPageRing];              // 16-key groups that nobody sees
   __shared__ int s_row[kPageRing][kGroups];        // first cache row of the group's keys (-1: none; -2: no more tiles)
   __shared__ Start s_start;
   __shared__ uint32_t s_tmem;
@@ -422,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       // positions of this warpgroup's first and last row bound where its masks are needed
       const int pa = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rem0);
       const int pb = k.start < 0 ? -1 : k.start + tok0 + token_of(kRows * w + rows - 1 + rem0);
-      float m = kNoMax, l = 0.f, ref = 0.f;
+      float m = kNoMax, v = kNoMax, l = 0.f, unit = 0.f;   // unit: 2^(m - v + kUnit)
       // 64 keys a step; the next step's scores are being computed meanwhile, in the other half of this row
       // tile's score columns
 #pragma unroll 1
@@ -443,8 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           kf[g + 1] = __uint_as_float(x.z);
           vf[g + 1] = __uint_as_float(x.w);
         }
-        const float vs = s_tile[slot].vmax;
-        const int unseen = s_tile[slot].unseen >> (4 * h) & 15;
+        const uint4 lv = lds128(smem_u32(&s_log[slot][4 * h]));
+        const int unseen = s_unseen[slot] >> (4 * h) & 15;
         // whether some key is hidden from some row: past its position, out of its window, without a page
         const bool hidden = j0 + 63 > pa || (a.window >= 0 && !(j0 > pb - a.window || j0 + 64 <= a.sinks)) || unseen;
         if (hidden) {
@@ -476,34 +475,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           tmem_wait_st();
           tmem_ld_32x32b_x32(tH, s0);
         }
-        float mx = kNoMax;
-        auto top = [&](const uint32_t* s, float f0, float f1) {
+        float mx = kNoMax, vx = kNoMax;            // the largest score, the largest contribution
+        auto top = [&](const uint32_t* s, float f0, float f1, uint32_t l0, uint32_t l1) {
 #pragma unroll
           for (int g = 0; g < 2; g++) {
             const uint32_t* z = s + 16 * g;
-            float u = max3(z[0], z[1], z[2]), v = max3(z[3], z[4], z[5]);
+            float u = max3(z[0], z[1], z[2]), w = max3(z[3], z[4], z[5]);
             u = max3(u, z[6], z[7]);
-            v = max3(v, z[8], z[9]);
+            w = max3(w, z[8], z[9]);
             u = max3(u, z[10], z[11]);
-            v = max3(v, z[12], z[13]);
+            w = max3(w, z[12], z[13]);
             u = max3(u, z[14], z[15]);
-            mx = fmaxf(mx, fmaxf(u, v) * (g ? f1 : f0));
+            u = fmaxf(u, w) * (g ? f1 : f0);
+            mx = fmaxf(mx, u);
+            vx = fmaxf(vx, u + __uint_as_float(g ? l1 : l0));
           }
         };
         tmem_wait_ld();
         tmem_ld_32x32b_x32(tH + 32, s1);
-        top(s0, kf[0], kf[1]);
+        top(s0, kf[0], kf[1], lv.x, lv.y);
         tmem_wait_ld();
-        top(s1, kf[2], kf[3]);
-        // ---- raise the maximum or the value reference, and bring O along (its products must be done)
-        const bool raise = mx > m + kRaise, refer = vs > 2.f * ref || (vs > 0.f && vs < ref * (1.f / 64.f));
-        if (__any_sync(0xffffffffu, raise || refer)) {
-          const float m2 = fmaxf(m, mx), ref2 = refer ? vs : ref;
-          const float down = exp2_fast(m - m2);
-          const float by = ref2 > 0.f ? down * __fdividef(ref, ref2) : down;
-          l *= down;
+        top(s1, kf[2], kf[3], lv.z, lv.w);
+        // ---- raise the maxima, and bring O along (its products must be done)
+        if (__any_sync(0xffffffffu, mx > m + kRaise || vx > v + kRaise)) {
+          const float m2 = fmaxf(m, mx), v2 = fmaxf(fmaxf(v, vx), m2 - kLow);
+          const float by = exp2_fast(v - v2);
+          l *= exp2_fast(m - m2);
           m = m2;
-          ref = ref2;
+          v = v2;
+          unit = exp2_fast(m - v + kUnit);
           if (u > 2 * k.t0) {
             // the step before's (that these scores are there says that those before it are done, so this
             // barrier is at most one phase behind: a wait cannot tell more)
@@ -520,16 +520,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             }
           }
         }
-        // ---- weights: p = 2^(score - m); the row sum keeps p, the product gets p s_v / ref in fp16, over the
-        // scores that they came from
-        const float unit = ref > 0.f ? __fdividef(kWeightUnit, ref) : 0.f;
+        // ---- weights: p = 2^(score - m); the row sum keeps p, the product gets p s_v unit in fp16, over the
+        // scores that they came from. (A page that this row does not see may make the factor infinite: its p are 0.)
         const uint64_t nm = two(-m, -m);
         uint64_t l2[2] = {0ull, 0ull};
         uint32_t p[32];
         auto weigh = [&](const uint32_t* s, uint32_t* to, float f0, float f1, float w0, float w1) {
 #pragma unroll
           for (int g = 0; g < 2; g++) {
-            const float fg = g ? f1 : f0, wg = (g ? w1 : w0) * unit;
+            const float fg = g ? f1 : f0, wg = fminf((g ? w1 : w0) * unit, FLT_MAX);
             const uint64_t fg2 = two(fg, fg), wg2 = two(wg, wg);
 #pragma unroll
             for (int y = 0; y < 8; y++) {
@@ -556,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       TILE_WAIT(bar.o_done[w][0], ((it - 1) >> 1) & 1);
       TILE_WAIT(bar.o_done[w][1], ((it - 1) >> 1) & 1);
       tc_fence_after();
-      const float back = ref * (1.f / kWeightUnit);
+      const float back = exp2_fast(v - m - kUnit);
       uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + ((size_t)(k.row0 + tok0 + my_tok) * a.H + k.head * G + my_head) * kHd);
       auto store = [&](int c, const float* o, float f) {             // 32 columns of this thread's row
         if (!live) return;
@@ -809,14 +808,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
 #pragma unroll 1
           for (int i = 0; i < kAhead && i0 >= k.t0 && i0 + i < k.t1; i++, t++) {
             if (t >= kAhead) TILE_WAIT(bar.page_empty[t % kAhead], (t / kAhead - 1) & 1);
-            float vmax = sc.y;
-#pragma unroll
-            for (int o = 1; o < kGroups; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
             const unsigned unseen = __ballot_sync(0xffffffffu, y < 0) >> (i * kGroups) & ((1u << kGroups) - 1);
             if (lane / kGroups == i) {
               s_row[t % kPageRing][grp] = y;
               s_scale[t % kPageRing][grp] = sc;
-              if (grp == 0) s_tile[t % kPageRing] = TileInfo{vmax, (int)unseen};
+              s_log[t % kPageRing][grp] = __log2f(fabsf(sc.y));
+              if (grp == 0) s_unseen[t % kPageRing] = (int)unseen;
             }
             warp_arrive(&bar.page_full[t % kAhead]);
           }
