@@ -92,3 +92,20 @@ def test_unlikely_keys_with_large_values(dev, decades, new):
         g = torch.Generator(device=dev).manual_seed(seed)
         cache["sv"] = 10.0 ** (decades * (torch.rand(cache["sv"].shape, device=dev, generator=g) - 0.5))
         check_rows(dev, b, cache, q)
+
+
+@pytest.mark.parametrize("new", FORMS)
+@pytest.mark.parametrize("apart", [10, 20, 28, 40])
+def test_one_page_of_unlikely_keys_decides(dev, apart, new):
+    """Keys of 2^-apart of the others' probability (jittered, no powers of two) whose values are 2^(apart + 5) times
+    as large: both kinds reach the output."""
+    b, cache, q = setup(dev, [192], [new], 16, 1, BF, 8)
+    q.fill_(1.0)
+    unit = math.log(2) / 128 * 0.97
+    cache["sk"].fill_(1.0)
+    cache["k"].zero_()
+    page = b.table[0][6].item()                            # 64 keys on from page 2
+    cache["k"][page] = -(apart - 2 + torch.arange(16, device=dev, dtype=torch.int8) % 5)[None, :, None]
+    cache["sv"].fill_(0.01)
+    cache["sv"][page] *= 2.0 ** (apart + 5)
+    check_rows(dev, b, cache, q, scale=unit)

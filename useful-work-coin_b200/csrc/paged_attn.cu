@@ -21,15 +21,17 @@
 //   1/sqrt(d) multiply the float32 sums. Keys lie on the M side, so the conversion serves every query
 //   row, and the order of dims and keys inside a fragment is chosen so that a thread reads 16-byte runs
 //   (conflict-free under the swizzle) and no shuffle moves K or V; P is transposed by movmatrix.
-//   Weights are 2^(score - m) with m 7 below the row's maximum when it was last looked at; m is raised only
-//   when a score passes it by 15, so most tiles neither reduce over lanes nor rescale. They stay below 2^15,
-//   inside fp16, which keeps 11 bits of those down to 2^-21 of the largest (2^-14 without the 7).
+//   Weights are 2^(score - m) s_v 2^(m - v), with m 7 below the row's maximum when it was last looked at and v as far
+//   below its largest score + log2 s_v; both are raised only when a key passes one by 15, so most tiles neither reduce
+//   over lanes nor rescale. They stay below 2^15, inside fp16, which keeps 11 bits of those down to 2^-21 of the row's
+//   largest contribution, however far apart the pages' scales are (2^-14 without the 7).
 //
 // Measured on B200 (a graph of calls): one sequence of 131071 tokens, 32 heads on 8: 58 us, 4.6 TB/s; 32
 // sequences of up to 8192: 59 us, 4.8 TB/s; 64 with a window of 1024: 40 us, 3.2 TB/s. A share's first tile comes
 // 6 us after the launch (metadata, pages, scales, the copy), and a unit's end takes 3 to 5 us (four warps' sums,
 // the part's write, the count, the join), which three CTAs an SM hide in part.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <mutex>
 #include <set>
@@ -48,7 +50,8 @@ constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kTile = 64;                    // keys per stage
 constexpr int kGroups = kTile / 16;          // 16-key groups: one warp's share, always inside one page
 constexpr int kStageBytes = 2 * kTile * kHd; // keys, then values
-constexpr float kHeadroom = 7.f, kRaise = 8.f;   // log2: of the largest weight when m is set; by which a later one may pass it
+constexpr float kHeadroom = 7.f, kRaise = 8.f;   // log2: of the largest weight when m and v are set; by which a later one may pass it
+constexpr float kLow = 116.f;                // v is no lower than m by more: 2^(m - v) is finite, 2^(v - m) not 0
 constexpr int kBatch = 8;                    // tiles whose page ids and scales are fetched at once
 constexpr int kUnitCost = 5;                 // what a unit costs beside its tiles, in tiles
 constexpr int kMinTiles = 4;                 // the least tiles of a CTA's share of the line (a join costs about as much)
@@ -332,11 +335,11 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           qpos[n][c] = rc < rows ? k.sp.start + rc / G : -1;
         }
       }
-      float m[NT][2], l[NT][2], o[NT][8][4];
+      float m[NT][2], v[NT][2], unit[NT][2], l[NT][2], o[NT][8][4];   // unit: 2^(m - v)
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        m[n][0] = m[n][1] = kNoMax;
-        l[n][0] = l[n][1] = 0.f;
+        m[n][0] = m[n][1] = v[n][0] = v[n][1] = kNoMax;
+        l[n][0] = l[n][1] = unit[n][0] = unit[n][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -351,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
         const int j0 = k.key(i) + 16 * warp;
         if (there && s_seen[st][warp]) {
           const float2 sc = s_scale[st][warp];
+          const float lv = __log2f(fabsf(sc.y));
           const uint32_t base = sm0 + st * kStageBytes;
           uint4 kw[4];
           kw[0] = lds128(base + koff0);
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) over |= sa[n][x] > m[n][x & 1] + (kHeadroom + kRaise);
+            for (int x = 0; x < 4; x++) over |= sa[n][x] > fminf(m[n][x & 1], v[n][x & 1] - lv) + (kHeadroom + kRaise);
           if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
@@ -409,10 +413,13 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                x = fmaxf(x - kHeadroom, m[n][c]);
-                const float f = exp2_fast(m[n][c] - x);
-                m[n][c] = x;
-                l[n][c] *= f;
+                x -= kHeadroom;
+                const float m2 = fmaxf(x, m[n][c]), v2 = fmaxf(fmaxf(x + lv, v[n][c]), m2 - kLow);
+                const float f = exp2_fast(v[n][c] - v2);
+                l[n][c] *= exp2_fast(m[n][c] - m2);
+                m[n][c] = m2;
+                v[n][c] = v2;
+                unit[n][c] = exp2_fast(m2 - v2);
 #pragma unroll
                 for (int d = 0; d < 8; d++) {
                   o[n][d][c] *= f;
@@ -423,16 +430,19 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           uint32_t pf[NT][2];
 #pragma unroll
           for (int n = 0; n < NT; n++) {
+            // (a page that a row does not see may make its factor infinite: the row's weights there are 0)
+            const float by[2] = {fminf(sc.y * unit[n][0], FLT_MAX), fminf(sc.y * unit[n][1], FLT_MAX)};
 #pragma unroll
             for (int x = 0; x < 4; x++) {
               sa[n][x] = exp2_fast(sa[n][x] - m[n][x & 1]);
               l[n][x & 1] += sa[n][x];
+              sa[n][x] *= by[x & 1];
             }
             const __half2 p0 = __floats2half2_rn(sa[n][0], sa[n][1]), p1 = __floats2half2_rn(sa[n][2], sa[n][3]);
             pf[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&p0));
             pf[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&p1));
           }
-          // ---- O^T += s_v V^T P^T: dims 16 g + 2 i and 16 g + 2 i + 1 are rows g and g + 8 of product i
+          // ---- O^T += V^T P^T: dims 16 g + 2 i and 16 g + 2 i + 1 are rows g and g + 8 of product i
           const uint32_t r0[4] = {vw[0].x, vw[0].y, vw[0].z, vw[0].w}, r1[4] = {vw[1].x, vw[1].y, vw[1].z, vw[1].w};
           const uint32_t r2[4] = {vw[2].x, vw[2].y, vw[2].z, vw[2].w}, r3[4] = {vw[3].x, vw[3].y, vw[3].z, vw[3].w};
 #pragma unroll
@@ -443,13 +453,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
               const uint32_t u = __byte_perm(r0[w], r1[w], sel) ^ 0x80808080u, v = __byte_perm(r2[w], r3[w], sel) ^ 0x80808080u;
               const uint32_t af[4] = {i8_half2(u, 0x4140), i8_half2(u, 0x4342), i8_half2(v, 0x4140), i8_half2(v, 0x4342)};
 #pragma unroll
-              for (int n = 0; n < NT; n++) {
-                const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-                float d[4];
-                mma_f16(d, af, pf[n], zero);
-#pragma unroll
-                for (int x = 0; x < 4; x++) o[n][2 * w + y][x] = fmaf(d[x], sc.y, o[n][2 * w + y][x]);
-              }
+              for (int n = 0; n < NT; n++) mma_f16(o[n][2 * w + y], af, pf[n], o[n][2 * w + y]);
             }
           }
         }
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           float L = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; w++) L += s_l[w][r] * exp2_fast(s_m[w][r] - M);
-          const float f = exp2_fast(m[n][c] - M);
+          const float f = exp2_fast(v[n][c] - M);        // to the units of M
           m[n][c] = M;
           l[n][c] = L;
 #pragma unroll
