@@ -85,6 +85,29 @@ def test_queries_up_to_the_largest(dev, e):
     check_rows(dev, b, cache, (q.double() * up).to(BF), scale=math.ldexp(1 / math.sqrt(D), 62 - e))
 
 
+@pytest.mark.parametrize("new", [1, 20])
+def test_held_integers_of_minus_128(dev, new):
+    """An old token's integer is rounded in its new scale and not clamped, on either side of the quick quotient."""
+    from uwc_b200 import paged
+    ps, n = 64, 60
+    for s0 in (127.5 / 128, 0.7, 0.9999):                  # -128 s0 / s: a tie, and two that are none
+        b = Batch([n], [new], ps)
+        cache = paged.new_cache(b.pages, 2, ps, dev)
+        for name in ("k", "v"):
+            cache[name][:] = (torch.arange(cache[name].numel(), device=dev) % 256 - 128).to(torch.int8).view(cache[name].shape)
+        cache["sk"].fill_(s0)
+        cache["sv"].fill_(s0)
+        x = torch.zeros(new, 2, D, dtype=BF, device=dev)
+        x[0, :, 0] = 127.0                                 # the new scale is 1
+        cosd, sind = torch.ones(n, D, device=dev), torch.zeros(n, D, device=dev)
+        f = x.float().cpu().numpy()
+        want = append_plain(f, f, numpy_cache(cache), b, cosd.cpu().numpy(), sind.cpu().numpy())
+        paged.append(x, x, cache, *b.device(dev), b.max_new, cosd, sind)
+        for name in ("sk", "sv", "k", "v"):
+            assert np.array_equal(cache[name].cpu().numpy(), want[name]), (s0, name)
+        assert (cache["v"][int(b.table[0, 0]), :, :n - new] == -128).any() == (s0 > 0.99)
+
+
 @pytest.mark.parametrize("most", [1, 8, 60])
 @pytest.mark.parametrize("cu", [(5, -2 ** 31), (1, 2 - 2 ** 31), (2 ** 31 - 1, -2 ** 31), (2 ** 31 - 1, 2 ** 31 - 1 - 60),
                                 (-2 ** 31, 2 ** 31 - 1), (-2 ** 31, -2 ** 31)], ids=str)

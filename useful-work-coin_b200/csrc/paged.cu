@@ -130,23 +130,24 @@ __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= FLT_MAX ? a : 0.f;
 }
-// Four values as clamp(rint(fdiv(x, s)), +-127), NaN as 0.
-__device__ __forceinline__ uint32_t quant4_exact(float4 x4, float s) {
+// Four values as clamp(rint(fdiv(x, s)), least, 127), NaN as 0. least: -127 for new values; -128 for held ones, whose
+// integers a caller may have written.
+__device__ __forceinline__ uint32_t quant4_exact(float4 x4, float s, float least) {
   const float x[4] = {x4.x, x4.y, x4.z, x4.w};
   uint32_t o = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const float v = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f) : 0.f;
+    const float v = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), least), 127.f) : 0.f;
     const int q = x[i] == x[i] ? (int)v : 0;
     o |= (uint32_t)(q & 255) << (8 * i);
   }
   return o;
 }
 // The same without the divisions (half of the kernel's instructions) where that cannot change a bit: inv is
-// 1 / s, so x inv is within 1e-4 of the quotient (|quotient| <= 127), and both round to the same integer
+// 1 / s, so x inv is within 1e-4 of the quotient (|quotient| <= 128), and both round to the same integer
 // unless it lies that near to a half. 1.5 2^23 + x inv has the integer in its low byte. Infinities, NaN and
 // an infinite inv leave a NaN, which fails the test too.
-__device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv) {
+__device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv, float least = -127.f) {
   constexpr float kMagic = 12582912.f;
   uint32_t t[4];
   float off = 0.f;
@@ -156,7 +157,7 @@ __device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv) {
     t[i] = __float_as_uint(z);
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(off) : "f"(fabsf(fmaf(x[i], inv, kMagic - z))));
   }
-  if (!(off < 0.4999f)) return quant4_exact(make_float4(x[0], x[1], x[2], x[3]), s);
+  if (!(off < 0.4999f)) return quant4_exact(make_float4(x[0], x[1], x[2], x[3]), s, least);
   return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 __device__ __forceinline__ float inverse(float s) { return s > 1e-30f ? __frcp_rn(s) : __int_as_float(0x7f800000); }
@@ -311,7 +312,7 @@ __device__ __forceinline__ void requantize(const PageUnit& u, float s0, float s,
       float f[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) f[i] = __fmul_rn((float)(int8_t)(y[k] >> (8 * i)), s0);
-      y[k] = quant4(f, s, inv);
+      y[k] = quant4(f, s, inv, -128.f);
     }
     d[w] = make_uint4(y[0], y[1], y[2], y[3]);
   }
