@@ -85,6 +85,20 @@ def test_queries_up_to_the_largest(dev, e):
     check_rows(dev, b, cache, (q.double() * up).to(BF), scale=math.ldexp(1 / math.sqrt(D), 62 - e))
 
 
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_pages_of_zero_keys_under_large_queries(dev, new):
+    """A page whose key scale is 0 (or almost) adds nothing to a score, however large the query."""
+    from test_gpu_paged_scales import check_rows
+    for small in (0.0, 1e-40, 3e-39):
+        b = Batch([200], [new], 16, seed=new)
+        cache = random_cache(b, 1, dev, new, spread=0.0)
+        q, _, _ = fused_rows(new, 2, 1, BF, dev, new)
+        cache["sk"] *= 1e-34
+        for at in (1, 5, 9):
+            cache["sk"][b.table[0][at].item()] = small
+        check_rows(dev, b, cache, (q.double() * 1e34).to(BF))
+
+
 @pytest.mark.parametrize("new", [1, 20])
 def test_held_integers_of_minus_128(dev, new):
     """An old token's integer is rounded in its new scale and not clamped, on either side of the quick quotient."""

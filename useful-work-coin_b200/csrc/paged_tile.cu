@@ -63,6 +63,8 @@ constexpr int kItemCost = 2;                 // what an item costs beside its ti
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 // 128 dims; values are stored key by key: B is MN-major
 constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(kHd >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+constexpr float kNoScore = 1.4e-45f;         // the factor of scores in pages of (almost) zero keys: not 0, so that -inf stays
+                                             // -inf, and the smallest there is, since a bf16 query may reach 1e38
 constexpr float kRaise = 4.f;                // log2 by which a score may pass the running maximum
 constexpr float kUnit = 10.f;                // log2 of the largest contribution's fp16 weight when v was set
 constexpr float kLow = 116.f;                // v is no lower than m by more: 2^(m - v + kUnit) is finite, 2^(v - m - kUnit) not 0
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         auto look = [&](int i0, int& y, float2& sc) {
           const int i = i0 + lane / kGroups, j = k.key(i) + 16 * grp;
           y = -1;
-          sc = make_float2(1e-37f, 0.f);
+          sc = make_float2(kNoScore, 0.f);
           if (i < k.t1 && k.seen(j, 16)) {
             const int page = page_at(a.b, a.c, k.seq, j >> a.c.lg);
             if (page < 0) {
@@ -794,13 +796,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             } else {
               const int ph = page * Hkv + k.head;      // rows of the pool fit an int: the host checks
               y = ph * ps + (j & (ps - 1));
-              // the factor of scores is not 0, so that a hidden score stays -inf
-              sc = make_float2(fmaxf(__ldg(a.c.sk + ph) * qmul, 1e-37f), __ldg(a.c.sv + ph));
+              sc = make_float2(fmaxf(__ldg(a.c.sk + ph) * qmul, kNoScore), __ldg(a.c.sv + ph));
             }
           }
         };
         int y = -1, ny;
-        float2 sc = make_float2(1e-37f, 0.f), nsc;
+        float2 sc = make_float2(kNoScore, 0.f), nsc;
         // the look-up of four tiles ahead of their hand-over
 #pragma unroll 1
         for (int i0 = k.t0 - kAhead; i0 < k.t1; i0 += kAhead) {
