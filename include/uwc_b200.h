@@ -48,8 +48,9 @@ extern "C" {
 
 /* Test hooks of the error path (no counterpart in the reference). UWC_HOOK_WAIT_NS sets the bound of
  * every wait inside the GEMM kernels (value in ns; 0 restores the default of 1 s);
- * UWC_HOOK_WITHHOLD = 1 makes later GEMM launches issue no copies, so their first wait runs out and
- * the kernel unwinds with UWC_DEV_TIMEOUT in uwc_device_status (0 restores normal launches);
+ * UWC_HOOK_WITHHOLD = 1 makes later GEMM launches issue no copies, and every second CTA of later paged
+ * attention launches fetch no pages, so that their first wait runs out and the kernel unwinds with
+ * UWC_DEV_TIMEOUT in uwc_device_status (0 restores normal launches);
  * UWC_HOOK_STREAM_PDL = 0 launches the weight-streaming GEMM and the few-row quantizers without
  * programmatic dependent launch (1, the default, lets them start while the previous kernel of the
  * stream finishes); UWC_HOOK_TP_TWO_PHASE = w (1..9) runs uwc_gemm_stream_tp's exchange as

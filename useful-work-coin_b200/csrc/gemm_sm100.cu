@@ -1132,6 +1132,7 @@ bool split_k(int m, int n) {
 }  // namespace
 
 uint64_t uwc_wait_ns() { return g_wait_ns.load(); }
+int uwc_withhold() { return g_withhold.load(); }
 
 extern "C" int uwc_test_hook(int hook, long long value) {
   if (hook == UWC_HOOK_WAIT_NS && value >= 0) {

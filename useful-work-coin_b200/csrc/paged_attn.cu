@@ -70,6 +70,7 @@ struct TokenArgs {
   float* part_o;           // (2 grid, 8 NT, 128): a CTA's two partial units, unnormalized
   float2* part_ml;         // (2 grid, 8 NT): m (log2), sum
   uint32_t* counters;      // (grid): finished parts of the unit that starts in this CTA; left zero
+  int withhold;            // 1: every other CTA copies no pages (a test's hook), so that its waits run out
 };
 
 // A sequence's tiles: one pass over the keys for all its new tokens.
@@ -221,7 +222,10 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
           for (int i = 0; i < kBatch && tb + i < end; i++, it++) {
             const int st = it % ST;
             const uint32_t use = (uint32_t)(it / ST);
-            if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[st], (use - 1) & 1, &s_abort, a.status))) {
+            // A wait that ran out in another warp counts here too: its stage was given back without its copies, so
+            // the barrier's phase is not over and takes no second arrival.
+            if (use > 0 && (!__all_sync(0xffffffffu, mbar_wait(&empty[st], (use - 1) & 1, &s_abort, a.status)) ||
+                            __any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort)))) {
               // give up: let the copies in flight land (bounded), then leave
 #pragma unroll 1
               for (int x = max(0, it - ST); x < it; x++)
@@ -245,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, TokenCfg<NT>::kCtas)
             __syncwarp();
             if (elect_one()) mbar_expect_tx(&full[st], (uint32_t)(boxes * 2 * box * kHd));
             __syncwarp();
-            if (issue) {
+            if (issue && !(ta.withhold & blockIdx.x & 1)) {
               const int y = (bpage * Hkv + h) * ps + (j0 & (ps - 1));
               uint8_t* dst = sm + st * kStageBytes + grp * 16 * kHd;
               tma_load_2d(dst, &mapK, &full[st], 0, y);
@@ -682,6 +686,7 @@ int launch_token(const AttnArgs& a, int max_len, uint8_t* ws, cudaStream_t st) {
   ta.counters = reinterpret_cast<uint32_t*>(ws);
   ta.part_o = reinterpret_cast<float*>(ws + kCounterBytes);
   ta.part_ml = reinterpret_cast<float2*>(ta.part_o + (size_t)grid * 2 * 8 * NT * kHd);
+  ta.withhold = uwc_withhold();
   k_paged_token<T, NT><<<grid, kThreads, TokenCfg<NT>::kSmem, st>>>(ta, mk, mv);
   uwc_count_launch();
   return uwc_launch_status();
