@@ -1,6 +1,7 @@
 """Paged attention whose waits run out, with no fault: the hook makes every second CTA fetch no pages. The call
 returns, the status says so, the workspace's counters are zero as after any call, and the next call is right."""
 import math
+import time
 
 import pytest
 import torch
@@ -73,3 +74,19 @@ def test_the_kept_workspace_survives_a_timeout(dev, withhold, new):
     withhold(False)
     for _ in range(2):
         assert torch.equal(paged.attention(*args), want)
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_a_wait_takes_about_a_second(dev, withhold, new):
+    from uwc_b200 import _lib, paged
+    b = Batch([3000], [new], 64)
+    cache = random_cache(b, 2, dev)
+    q = fused_rows(b.rows, 8, 2, BF, dev, 0)[0]
+    args = (q, cache, *b.device(dev), b.max_new, b.max_len)
+    paged.attention(*args)
+    assert _lib.device_status(clear=True) == 0
+    withhold(True)
+    t = time.perf_counter()
+    paged.attention(*args)
+    assert _lib.device_status(clear=True) == _lib.DEV_TIMEOUT
+    assert 0.02 < time.perf_counter() - t < 8              # one wait, of a second or so, and the way out

@@ -74,6 +74,7 @@ struct TileArgs {
   float* part_o;           // (2 grid, 2, 32, 128, 4): a CTA's two partial items by row tile, four columns, row; unnormalized
   float2* part_ml;         // (2 grid, 256): running maximum (log2), sum
   uint32_t* counters;      // (grid, 2): finished parts of the item that starts in this CTA; left zero
+  int withhold;            // 1: every other CTA looks no pages up (a test's hook), so that its waits run out
 };
 
 // 256 rows of one (sequence, KV head): tokens t0 .. t1 have rows in it.
@@ -777,6 +778,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
         if (lane == 0) mbar_arrive(&bar.piece_full[slot]);
         if (end) break;
       }
+    } else if (warp == 14 && (ta.withhold & blockIdx.x & 1)) {
+      // the hook: no tile is handed over
     } else if (warp == 14) {
       // ---------------------------------------------------------------- the pages: a lane a 16-key group, four tiles at once
       const int grp = lane & (kGroups - 1);
@@ -949,6 +952,7 @@ int uwc_paged_tile_launch(const AttnArgs* a, int dtype, int max_len, void* works
   ta.counters = reinterpret_cast<uint32_t*>(ws);
   ta.part_o = reinterpret_cast<float*>(ws + kCounterBytes);
   ta.part_ml = reinterpret_cast<float2*>(ta.part_o + (size_t)grid * 4 * kRows * kHd);
+  ta.withhold = uwc_withhold();
   const void* fn = dtype == UWC_T_BF16 ? (const void*)k_paged_tile<__nv_bfloat16> : (const void*)k_paged_tile<__half>;
   const int rc = uwc_paged_allow_smem(fn, kSmem);
   if (rc != UWC_OK) return rc;
