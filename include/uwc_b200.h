@@ -480,7 +480,8 @@ int uwc_paged_gather(const int8_t* kc, const float* sk, const int8_t* vc, const 
  * H a multiple of Hkv (head h reads KV head h / (H / Hkv)); out (rows, H, 128) contiguous, in dtype.
  * softmax(scale q . k) in float32, scale finite; a row that sees no key is zero. No atomics touch a result: the same
  * call gives the same bits. workspace: uwc_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
- * whose first 4096 are zero before its first use (counters; every call leaves them zero). Calls that
+ * whose first 4096 are zero before its first use (counters; every call leaves them zero, one that raised
+ * UWC_DEV_TIMEOUT too). Calls that
  * overlap on the GPU must not share one. */
 uint64_t uwc_paged_attention_workspace_bytes(int seqs, int max_new, int max_len, int H, int Hkv, int window,
                                              int sinks);

@@ -25,12 +25,12 @@ def withhold(dev):
     assert _lib.device_status(clear=True) == 0
 
 
-# one long unit in many parts, units of every length
-SHAPES = [([20000], [1], 4, 1), ([9000, 20, 3000], [3, 1, 4], 8, 2)]
+# one long unit in many parts, units of every length, many short items (whole ones among them)
+SHAPES = [([20000], [1], 4, 1), ([9000, 20, 3000], [3, 1, 4], 8, 2), ([9000, 130], [300, 130], 4, 2), ([700] * 40, [40] * 40, 8, 2)]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("lens,new,H,Hkv", SHAPES, ids=["token", "drafts"])
+@pytest.mark.parametrize("lens,new,H,Hkv", SHAPES, ids=["token", "drafts", "chunks", "prompts"])
 def test_counters_are_zero_after_a_timeout(dev, withhold, lens, new, H, Hkv, dtype):
     from uwc_b200 import _lib
     L, b = _lib.lib(), Batch(lens, new, 64, seed=1)
@@ -59,7 +59,7 @@ def test_counters_are_zero_after_a_timeout(dev, withhold, lens, new, H, Hkv, dty
     assert torch.equal(call(), want) and not ws[:4096].any()
 
 
-@pytest.mark.parametrize("new", [1])
+@pytest.mark.parametrize("new", [1, 60])
 def test_the_kept_workspace_survives_a_timeout(dev, withhold, new):
     """paged.attention's own workspace, which is kept for the stream."""
     from uwc_b200 import _lib, paged

@@ -73,7 +73,7 @@ struct TileArgs {
   AttnArgs a;
   float* part_o;           // (2 grid, 2, 32, 128, 4): a CTA's two partial items by row tile, four columns, row; unnormalized
   float2* part_ml;         // (2 grid, 256): running maximum (log2), sum
-  uint32_t* counters;      // (grid, 2): finished parts of the item that starts in this CTA; left zero
+  uint32_t* counters;      // (grid, 2): finished parts of the item that starts in this CTA; the last brings it back to zero
   int withhold;            // 1: every other CTA looks no pages up (a test's hook), so that its waits run out
 };
 
@@ -320,6 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   __shared__ Start s_start;
   __shared__ uint32_t s_tmem;
   __shared__ int s_last[2];
+  __shared__ int3 s_part[2];                       // the CTA's parts of items that others share: rows, b0, b1; [1]: starts here
+  __shared__ int s_counted[2][2], s_gave_up;       // those that are counted, by row tile; whether a wait ran out
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smQ = smem_u32(sm), smK = smQ + 2 * kOperand, smV = smK + 2 * kOperand;
   if (tid == 0) {
@@ -338,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       mbar_init(&bar.wg[i], 4);
     }
     mbar_init(&bar.fin, 2);
+    s_counted[0][0] = s_counted[0][1] = s_counted[1][0] = s_counted[1][1] = s_gave_up = s_part[0].x = s_part[1].x = 0;
     for (int i = 0; i < kPieces; i++) {
       mbar_init(&bar.piece_full[i], 1);
       mbar_init(&bar.piece_empty[i], 11);
@@ -603,9 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       TILE_WAIT(bar.wg[w], wgp & 1);
       wgp++;
       if (r == 0) {
-        const uint32_t arrived = atomicAdd(&ta.counters[2 * b0 + w], 1u);
-        s_last[w] = arrived == (uint32_t)(b1 - b0);
-        if (s_last[w]) ta.counters[2 * b0 + w] = 0;
+        s_last[w] = atomicInc(&ta.counters[2 * b0 + w], b1 - b0) == (uint32_t)(b1 - b0);
+        s_counted[w][b0 == (int)blockIdx.x] = 1;
         __threadfence();
       }
       warp_arrive(&bar.wg[w]);
@@ -728,10 +730,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
       Start p = s_start;
       Span sp = batch.span(p.s);
       int blks = batch.blocks(sp);
+      bool quiet = false;
 #pragma unroll 1
       for (uint32_t n = 0;; n++) {
         const int slot = n % kPieces;
-        if (n >= kPieces) TILE_WAIT(bar.piece_empty[slot], (n / kPieces - 1) & 1);
+        // after a wait that ran out it goes on alone, for the parts that the CTA has to count
+        if (n >= kPieces && !quiet && !warp_wait(&bar.piece_empty[slot], (n / kPieces - 1) & 1)) {
+          quiet = true;
+          if (lane == 0) {
+            set_status(a.status, UWC_DEV_TIMEOUT);
+            s_gave_up = 1;
+          }
+        }
         Piece& k = s_piece[slot];
         bool end = true;
 #pragma unroll 1
@@ -740,19 +750,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
           const int all = kItemCost + it.total, u1 = min(all, p.u0 + p.left);
           if (u1 > kItemCost) {                    // some of its tiles, not only its own cost
             end = false;
-            if (lane == 0) {
+            const int rows = min(2 * kRows, sp.n * G - 2 * kRows * p.blk);
+            const bool whole = p.u0 <= kItemCost && u1 == all;
+            // the CTAs before this one hold the item's tiles before t0, those after it the rest, `per` each
+            const int b0 = blockIdx.x - (p.u0 > kItemCost ? (uint32_t)(p.u0 - kItemCost - 1) / (uint32_t)p.per + 1 : 0);
+            const int b1 = blockIdx.x + (all > u1 ? (uint32_t)(all - u1 - 1) / (uint32_t)p.per + 1 : 0);
+            if (lane == 0 && !whole) s_part[b0 == (int)blockIdx.x] = make_int3(rows, b0, b1);
+            if (lane == 0 && !quiet) {
               k.first = 2 * kRows * p.blk;
-              k.rows = min(2 * kRows, sp.n * G - 2 * kRows * p.blk);
+              k.rows = rows;
               k.row0 = sp.row0;
               k.seq = p.s;
               k.head = p.h;
               k.start = sp.idle ? -1 : sp.start;
               k.t0 = max(p.u0 - kItemCost, 0);
               k.t1 = u1 - kItemCost;
-              k.whole = p.u0 <= kItemCost && u1 == all;
-              // the CTAs before this one hold the item's tiles before t0, those after it the rest, `per` each
-              k.b0 = blockIdx.x - (p.u0 > kItemCost ? (uint32_t)(p.u0 - kItemCost - 1) / (uint32_t)p.per + 1 : 0);
-              k.b1 = blockIdx.x + (all > u1 ? (uint32_t)(all - u1 - 1) / (uint32_t)p.per + 1 : 0);
+              k.whole = whole;
+              k.b0 = b0;
+              k.b1 = b1;
               k.lo = it.lo;
               k.hi = it.hi;
               k.sink_end = it.sink_end;
@@ -773,9 +788,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
             }
           }
         }
-        if (end && lane == 0) k.rows = 0;
+        if (end && !quiet && lane == 0) k.rows = 0;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.piece_full[slot]);
+        if (lane == 0 && !quiet) mbar_arrive(&bar.piece_full[slot]);
         if (end) break;
       }
     } else if (warp == 14 && (ta.withhold & blockIdx.x & 1)) {
@@ -905,7 +920,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   }
   if (false) {
   timeout:
-    if (lane == 0) set_status(a.status, UWC_DEV_TIMEOUT);
+    if (lane == 0) {
+      set_status(a.status, UWC_DEV_TIMEOUT);
+      s_gave_up = 1;
+    }
   }
   __syncwarp();
   if (warp == 12 || warp == 15) {
@@ -923,6 +941,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
   if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+    // parts that a wait which ran out left uncounted: their items' counters end at zero all the same, for the next
+    // call with this workspace (this one's rows are lost, as the status says)
+    if (s_gave_up && lane == 0)
+#pragma unroll 1
+      for (int i = 0; i < 4; i++)
+        if (s_part[i & 1].x > kRows * (i >> 1) && !s_counted[i >> 1][i & 1])
+          atomicInc(&ta.counters[2 * s_part[i & 1].y + (i >> 1)], s_part[i & 1].z - s_part[i & 1].y);
   }
 }
 
