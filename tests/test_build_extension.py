@@ -1,0 +1,36 @@
+"""build.py on hosts that differ from this one: without torch and with a torch that has no CUDA. No compiler is run."""
+import importlib.util
+import os
+import sys
+
+import pytest
+import torch
+from conftest import PKG_ROOT
+
+
+@pytest.fixture
+def build(monkeypatch, tmp_path):
+    spec = importlib.util.spec_from_file_location("uwc_build", os.path.join(PKG_ROOT, "build.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.commands = []
+
+    def run(cmd):
+        m.commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+    monkeypatch.setattr(m.subprocess, "check_call", run)
+    monkeypatch.setattr(m, "up_to_date", lambda: True)
+    monkeypatch.setattr(m, "EXT_OUT", str(tmp_path / "_paged.so"))
+    return m
+
+
+def test_a_host_without_torch_gets_the_library(build, monkeypatch, capsys):
+    monkeypatch.setitem(sys.modules, "torch", None)        # import torch: ImportError
+    assert build.build() == build.OUT and build.commands == []
+    assert "_paged.so is not built" in capsys.readouterr().err
+
+
+def test_a_torch_without_cuda_does_too(build, monkeypatch, capsys):
+    monkeypatch.setattr(torch.version, "cuda", None)
+    assert build.build() == build.OUT and build.commands == []
+    assert "_paged.so is not built" in capsys.readouterr().err

@@ -4,7 +4,8 @@
 
 Output: useful-work-coin_b200/uwc_b200/libuwcb200.so, linked against the static CUDA runtime so
 it loads on a machine without a GPU driver (the symbol-export test runs on CPU-only hosts), and beside
-it _paged.so, the torch side of uwc_b200.paged (C++, no device code), linked to it and to torch.
+it _paged.so, the torch side of uwc_b200.paged (C++, no device code), linked to it and to torch (where
+there is a CUDA build of torch).
 Nothing is compiled at import time: the product path refuses to run without this library.
 """
 from __future__ import annotations
@@ -34,15 +35,24 @@ EXT_SOURCE = "paged_torch.cpp"
 EXT_OUT = os.path.join(HERE, "uwc_b200", "_paged.so")
 
 
-def build_extension(force: bool = False, verbose: bool = False) -> str:
-    """The torch extension module: calls of the library from tensors."""
+def build_extension(force: bool = False, verbose: bool = False) -> str | None:
+    """The torch extension module: calls of the library from tensors. None where there is no CUDA torch to build it
+    for: the library, for C callers and the ctypes modules, needs nvcc alone."""
+    try:
+        import torch
+        found = torch.version.cuda is not None
+    except ImportError:
+        found = False
+    if not found:
+        print(f"{os.path.basename(EXT_OUT)} is not built: no CUDA build of torch here (only uwc_b200.paged and .serve need it)",
+              file=sys.stderr)
+        return None
     src = os.path.join(CSRC, EXT_SOURCE)
     inputs = [src, os.path.join(ROOT, "include", "uwc_b200.h")]
     if not force and os.path.exists(EXT_OUT) and all(os.path.getmtime(f) <= os.path.getmtime(EXT_OUT) for f in inputs):
         return EXT_OUT
     import sysconfig
 
-    import torch
     from torch.utils import cpp_extension
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
