@@ -1,4 +1,5 @@
-"""build.py on hosts that differ from this one: without torch and with a torch that has no CUDA. No compiler is run."""
+"""build.py on hosts that differ from this one: without torch, with a torch that has no CUDA, with nvcc on the PATH
+alone. No compiler is run."""
 import importlib.util
 import os
 import sys
@@ -34,3 +35,18 @@ def test_a_torch_without_cuda_does_too(build, monkeypatch, capsys):
     monkeypatch.setattr(torch.version, "cuda", None)
     assert build.build() == build.OUT and build.commands == []
     assert "_paged.so is not built" in capsys.readouterr().err
+
+
+def test_nvcc_on_the_path_gives_its_headers(build, monkeypatch, tmp_path):
+    cuda = tmp_path / "toolkit"
+    (cuda / "bin").mkdir(parents=True)
+    (cuda / "bin" / "nvcc").write_text("#!/bin/sh\n")
+    (cuda / "bin" / "nvcc").chmod(0o755)
+    (tmp_path / "links").mkdir()
+    (tmp_path / "links" / "nvcc").symlink_to(cuda / "bin" / "nvcc")
+    monkeypatch.setenv("CUDA_HOME", str(tmp_path / "none"))
+    for d in (cuda / "bin", tmp_path / "links"):
+        monkeypatch.setenv("PATH", f"{d}:/bin")
+        build.build_extension(force=True)
+        assert f"-isystem{cuda}/include" in build.commands[-1]
+    assert not [a for a in build.commands[-1] if a == "-isysteminclude"]

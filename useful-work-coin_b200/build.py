@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import shutil
 import subprocess
 import sys
 
@@ -28,7 +29,7 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", 
 
 def nvcc() -> str:
     cand = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
-    return cand if os.path.exists(cand) else "nvcc"
+    return cand if os.path.exists(cand) else shutil.which("nvcc") or "nvcc"
 
 
 EXT_SOURCE = "paged_torch.cpp"
@@ -54,8 +55,8 @@ def build_extension(force: bool = False, verbose: bool = False) -> str | None:
     import sysconfig
 
     from torch.utils import cpp_extension
-    cuda = os.path.dirname(os.path.dirname(nvcc()))
-    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], *[d for d in [cuda] if d != "/usr/include"]]
     libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = EXT_OUT + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
