@@ -1,5 +1,5 @@
 """build.py on hosts that differ from this one: without torch, with a torch that has no CUDA, with nvcc on the PATH
-alone. No compiler is run."""
+alone, and after a change of torch. No compiler is run."""
 import importlib.util
 import os
 import sys
@@ -22,6 +22,7 @@ def build(monkeypatch, tmp_path):
     monkeypatch.setattr(m.subprocess, "check_call", run)
     monkeypatch.setattr(m, "up_to_date", lambda: True)
     monkeypatch.setattr(m, "EXT_OUT", str(tmp_path / "_paged.so"))
+    monkeypatch.setattr(m, "EXT_STAMP", str(tmp_path / "b" / "stamp"))
     return m
 
 
@@ -50,3 +51,15 @@ def test_nvcc_on_the_path_gives_its_headers(build, monkeypatch, tmp_path):
         build.build_extension(force=True)
         assert f"-isystem{cuda}/include" in build.commands[-1]
     assert not [a for a in build.commands[-1] if a == "-isysteminclude"]
+
+
+def test_another_torch_is_a_reason_to_build(build, monkeypatch):
+    build.build_extension()
+    assert len(build.commands) == 1
+    build.build_extension()
+    assert len(build.commands) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build_extension()
+    assert len(build.commands) == 2
+    build.build_extension()
+    assert len(build.commands) == 2

@@ -34,6 +34,7 @@ def nvcc() -> str:
 
 EXT_SOURCE = "paged_torch.cpp"
 EXT_OUT = os.path.join(HERE, "uwc_b200", "_paged.so")
+EXT_STAMP = os.path.join(HERE, "_build", "paged_torch.stamp")   # the torch and the Python that it was built for
 
 
 def build_extension(force: bool = False, verbose: bool = False) -> str | None:
@@ -50,7 +51,9 @@ def build_extension(force: bool = False, verbose: bool = False) -> str | None:
         return None
     src = os.path.join(CSRC, EXT_SOURCE)
     inputs = [src, os.path.join(ROOT, "include", "uwc_b200.h")]
-    if not force and os.path.exists(EXT_OUT) and all(os.path.getmtime(f) <= os.path.getmtime(EXT_OUT) for f in inputs):
+    stamp = f"{torch.__version__} {os.path.dirname(torch.__file__)} {sys.version}"
+    if (not force and os.path.exists(EXT_OUT) and all(os.path.getmtime(f) <= os.path.getmtime(EXT_OUT) for f in inputs)
+            and os.path.exists(EXT_STAMP) and open(EXT_STAMP).read() == stamp):
         return EXT_OUT
     import sysconfig
 
@@ -66,6 +69,9 @@ def build_extension(force: bool = False, verbose: bool = False) -> str | None:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
     os.replace(tmp, EXT_OUT)
+    os.makedirs(os.path.dirname(EXT_STAMP), exist_ok=True)
+    with open(EXT_STAMP, "w") as f:
+        f.write(stamp)
     return EXT_OUT
 
 
