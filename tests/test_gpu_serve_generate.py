@@ -1,0 +1,30 @@
+"""PagedBatch.generate at its limits: prompts that cannot be served are refused before any is, what exactly fits is
+served, and a call that fails leaves the batch as it found it."""
+import pytest
+import torch
+
+from test_gpu_serve import model, prompts, status_clean  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(b, pages):
+    return not b.active() and sorted(b.pool.free) == list(range(pages)) and bool((b._table == -1).all())
+
+
+def test_a_bad_prompt_is_refused_before_any_is_served(dev, model):
+    from uwc_b200 import _lib
+    from uwc_b200.serve import PagedBatch
+    b = PagedBatch(model, 2, 96, pages=5, page_size=16, graph=False)
+    good = prompts(20, 3, 17, 33)
+    calls = []
+    real = b._rows
+    b._rows = lambda *a: (calls.append(1), real(*a))[1]
+    for bad, error in (([], ValueError), (prompts(95)[0], ValueError), (prompts(80)[0], _lib.UWCError)):
+        with pytest.raises(error):                          # empty; 95 + 5 - 1 of 96 tokens; 6 of 5 pages
+            b.generate(good + [bad], 5)
+        assert not calls and whole(b, 5)
+    out = b.generate(good, 5)
+    assert [len(t) for t in out] == [5] * 4 and whole(b, 5)
+    one = PagedBatch(model, 1, 96, page_size=16, graph=False)
+    assert [one.generate([p], 5)[0] for p in good] == out

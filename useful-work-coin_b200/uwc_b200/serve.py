@@ -233,23 +233,24 @@ class PagedBatch:
 
     def generate(self, prompts: list[list[int]], n_new: int) -> list[list[int]]:
         """n_new greedy tokens after each prompt, from a batch whose slots are all idle: sequences enter as slots
-        and pages come free."""
+        and pages come free. Prompts that cannot be served are refused before any is."""
         if self.active():
             raise UWCError("generate wants every slot idle")
         if n_new < 1:
             return [[] for _ in prompts]
+        need = [-(-(len(p) + n_new) // self.pool.page_size) for p in prompts]
+        for i, p in enumerate(prompts):
+            if not p or len(p) + n_new > self.max_len:
+                raise ValueError(f"prompt {i} is empty or, with {n_new} tokens to come, longer than {self.max_len}")
+            if need[i] > len(self.pool.free):
+                raise UWCError(f"prompt {i} needs {need[i]} pages, of {len(self.pool.free)}")
         out: list[list[int]] = [[] for _ in prompts]
         waiting, owner = list(range(len(prompts))), {}
         while waiting or owner:
             room, enter = len(self.pool.free), []
-            while waiting and len(enter) < self.len.count(-1):
-                need = -(-(len(prompts[waiting[0]]) + n_new) // self.pool.page_size)
-                if need > room:
-                    break
-                room -= need
+            while waiting and len(enter) < self.len.count(-1) and need[waiting[0]] <= room:
+                room -= need[waiting[0]]
                 enter.append(waiting.pop(0))
-            if not enter and not owner:
-                raise UWCError(f"prompt {waiting[0]} needs more pages or slots than are free")
             got = self.admit([prompts[i] for i in enter], reserve=n_new)
             owner.update(zip(got, enter))
             if not got:
