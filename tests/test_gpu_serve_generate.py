@@ -21,10 +21,25 @@ def test_a_bad_prompt_is_refused_before_any_is_served(dev, model):
     real = b._rows
     b._rows = lambda *a: (calls.append(1), real(*a))[1]
     for bad, error in (([], ValueError), (prompts(95)[0], ValueError), (prompts(80)[0], _lib.UWCError)):
-        with pytest.raises(error):                          # empty; 95 + 5 - 1 of 96 tokens; 6 of 5 pages
+        with pytest.raises(error):                          # empty; 95 + 4 of 96 tokens; 6 of 5 pages
             b.generate(good + [bad], 5)
         assert not calls and whole(b, 5)
     out = b.generate(good, 5)
     assert [len(t) for t in out] == [5] * 4 and whole(b, 5)
     one = PagedBatch(model, 1, 96, page_size=16, graph=False)
     assert [one.generate([p], 5)[0] for p in good] == out
+
+
+def test_what_exactly_fits_is_served(dev, model):
+    """The last token is answered and not cached: 90 + 7 - 1 of 96 tokens, and a page of 16 for 12 + 5 - 1."""
+    from uwc_b200.serve import PagedBatch
+    long, short = prompts(90)[0], prompts(12)[0]
+    b = PagedBatch(model, 1, 96, pages=6, page_size=16, graph=False)
+    out = b.generate([long], 7)[0]
+    with pytest.raises(ValueError):
+        b.generate([long], 8)
+    roomy = PagedBatch(model, 1, 200, page_size=16, graph=False)
+    assert len(out) == 7 and out == roomy.generate([long], 7)[0]
+    one = PagedBatch(model, 3, 96, pages=1, page_size=16, graph=False)
+    assert one.generate([short, short[:3], short], 5) == roomy.generate([short, short[:3], short], 5) and whole(one, 1)
+    assert one.generate([prompts(16)[0]], 1) == roomy.generate([prompts(16)[0]], 1)

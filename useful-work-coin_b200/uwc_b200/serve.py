@@ -238,10 +238,11 @@ class PagedBatch:
             raise UWCError("generate wants every slot idle")
         if n_new < 1:
             return [[] for _ in prompts]
-        need = [-(-(len(p) + n_new) // self.pool.page_size) for p in prompts]
+        more = n_new - 1                              # the last token is answered, not cached
+        need = [-(-(len(p) + more) // self.pool.page_size) for p in prompts]
         for i, p in enumerate(prompts):
-            if not p or len(p) + n_new > self.max_len:
-                raise ValueError(f"prompt {i} is empty or, with {n_new} tokens to come, longer than {self.max_len}")
+            if not p or len(p) + more > self.max_len:
+                raise ValueError(f"prompt {i} is empty or, with {more} tokens to cache, longer than {self.max_len}")
             if need[i] > len(self.pool.free):
                 raise UWCError(f"prompt {i} needs {need[i]} pages, of {len(self.pool.free)}")
         out: list[list[int]] = [[] for _ in prompts]
@@ -251,7 +252,7 @@ class PagedBatch:
             while waiting and len(enter) < self.len.count(-1) and need[waiting[0]] <= room:
                 room -= need[waiting[0]]
                 enter.append(waiting.pop(0))
-            got = self.admit([prompts[i] for i in enter], reserve=n_new)
+            got = self.admit([prompts[i] for i in enter], reserve=more)
             owner.update(zip(got, enter))
             if not got:
                 got = self.step()
