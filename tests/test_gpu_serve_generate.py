@@ -43,3 +43,40 @@ def test_what_exactly_fits_is_served(dev, model):
     one = PagedBatch(model, 3, 96, pages=1, page_size=16, graph=False)
     assert one.generate([short, short[:3], short], 5) == roomy.generate([short, short[:3], short], 5) and whole(one, 1)
     assert one.generate([prompts(16)[0]], 1) == roomy.generate([prompts(16)[0]], 1)
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 5])
+def test_a_call_that_fails_leaves_the_batch_as_it_was(dev, model, at):
+    """An exception in the at-th pass through the model, of an admission or of a step: no slot and no page is lost."""
+    from uwc_b200.serve import PagedBatch
+    b = PagedBatch(model, 2, 96, pages=8, page_size=16, graph=False)
+    ps = prompts(40, 3, 17, 33)
+    want = b.generate(ps, 4)
+    real, seen = b._greedy, []
+
+    def failing(x):
+        seen.append(1)
+        if len(seen) == at + 1:
+            raise MemoryError("planted")
+        return real(x)
+    b._greedy = failing
+    with pytest.raises(MemoryError):
+        b.generate(ps, 4)
+    assert len(seen) == at + 1 and whole(b, 8)
+    b._greedy = real
+    assert b.generate(ps, 4) == want and whole(b, 8)
+
+
+def test_an_admission_that_fails_takes_nothing(dev, model):
+    from uwc_b200.serve import PagedBatch
+    b = PagedBatch(model, 3, 96, pages=8, page_size=16, graph=False)
+    ps = prompts(40, 20)
+    b.admit(ps[:1])
+    free = list(b.pool.free)
+    real, b._greedy = b._greedy, None                       # not callable
+    with pytest.raises(TypeError):
+        b.admit(ps[1:], reserve=3)
+    b._greedy = real
+    assert b.active() == [0] and sorted(b.pool.free) == sorted(free) and bool((b._table[1:] == -1).all())
+    b.admit(ps[1:])
+    assert b.active() == [0, 1] and list(b.step()) == [0, 1]

@@ -148,15 +148,21 @@ class PagedBatch:
         if not prompts:
             return {}
         self._hold(idle, [len(p) + reserve for p in prompts])
-        last = [None] * len(prompts)
-        for c0 in range(0, max(map(len, prompts)), chunk):
-            part = [i for i, p in enumerate(prompts) if len(p) > c0]
-            x = self._ragged([idle[i] for i in part], [prompts[i][c0:c0 + chunk] for i in part], [c0] * len(part))
-            end = 0
-            for i in part:
-                end += len(prompts[i][c0:c0 + chunk])
-                last[i] = x[end - 1]
-        tok = self._greedy(torch.stack(last))
+        try:
+            last = [None] * len(prompts)
+            for c0 in range(0, max(map(len, prompts)), chunk):
+                part = [i for i, p in enumerate(prompts) if len(p) > c0]
+                x = self._ragged([idle[i] for i in part], [prompts[i][c0:c0 + chunk] for i in part], [c0] * len(part))
+                end = 0
+                for i in part:
+                    end += len(prompts[i][c0:c0 + chunk])
+                    last[i] = x[end - 1]
+            tok = self._greedy(torch.stack(last))
+        except BaseException:
+            for s in idle:
+                self.pool.give_back(s)
+            self._table.copy_(self.pool.table())
+            raise
         where = torch.tensor(idle, device=self.model.device)
         self._tok[where] = tok
         self._start[where] = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=self.model.device)
@@ -247,18 +253,22 @@ class PagedBatch:
                 raise UWCError(f"prompt {i} needs {need[i]} pages, of {len(self.pool.free)}")
         out: list[list[int]] = [[] for _ in prompts]
         waiting, owner = list(range(len(prompts))), {}
-        while waiting or owner:
-            room, enter = len(self.pool.free), []
-            while waiting and len(enter) < self.len.count(-1) and need[waiting[0]] <= room:
-                room -= need[waiting[0]]
-                enter.append(waiting.pop(0))
-            got = self.admit([prompts[i] for i in enter], reserve=more)
-            owner.update(zip(got, enter))
-            if not got:
-                got = self.step()
-            for s, t in got.items():
-                out[owner[s]].append(t)
-            for s in [s for s, i in owner.items() if len(out[i]) == n_new]:
+        try:
+            while waiting or owner:
+                room, enter = len(self.pool.free), []
+                while waiting and len(enter) < self.len.count(-1) and need[waiting[0]] <= room:
+                    room -= need[waiting[0]]
+                    enter.append(waiting.pop(0))
+                got = self.admit([prompts[i] for i in enter], reserve=more)
+                owner.update(zip(got, enter))
+                if not got:
+                    got = self.step()
+                for s, t in got.items():
+                    out[owner[s]].append(t)
+                for s in [s for s, i in owner.items() if len(out[i]) == n_new]:
+                    self.release(s)
+                    del owner[s]
+        finally:                                      # a call that failed leaves no slot occupied
+            for s in self.active():
                 self.release(s)
-                del owner[s]
         return out
