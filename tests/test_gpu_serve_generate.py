@@ -80,3 +80,13 @@ def test_an_admission_that_fails_takes_nothing(dev, model):
     assert b.active() == [0] and sorted(b.pool.free) == sorted(free) and bool((b._table[1:] == -1).all())
     b.admit(ps[1:])
     assert b.active() == [0, 1] and list(b.step()) == [0, 1]
+
+
+def test_chunks_and_reserves_are_checked(dev, model):
+    """A reserve below 0 took fewer pages than the prompt fills."""
+    from uwc_b200.serve import PagedBatch
+    b = PagedBatch(model, 2, 96, pages=8, page_size=16, graph=False)
+    for bad in (dict(chunk=0), dict(chunk=-5), dict(reserve=-1), dict(reserve=-40)):
+        with pytest.raises(ValueError):
+            b.admit(prompts(40), **bad)
+        assert whole(b, 8)

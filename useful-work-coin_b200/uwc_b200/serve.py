@@ -145,6 +145,8 @@ class PagedBatch:
             raise UWCError(f"{len(prompts)} prompts, {len(idle)} idle slots")
         if any(not 0 < len(p) or len(p) + reserve > self.max_len for p in prompts):
             raise ValueError(f"a prompt is empty or, with {reserve} tokens to come, longer than {self.max_len}")
+        if chunk < 1 or reserve < 0:
+            raise ValueError(f"chunk {chunk}, reserve {reserve}")
         if not prompts:
             return {}
         self._hold(idle, [len(p) + reserve for p in prompts])
