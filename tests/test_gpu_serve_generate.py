@@ -90,3 +90,19 @@ def test_chunks_and_reserves_are_checked(dev, model):
         with pytest.raises(ValueError):
             b.admit(prompts(40), **bad)
         assert whole(b, 8)
+
+
+@pytest.mark.parametrize("bad", [-1, 1024, 2 ** 31, -2 ** 40])
+def test_tokens_that_the_model_has_not_are_refused(dev, model, bad):
+    from uwc_b200.serve import PagedBatch
+    b = PagedBatch(model, 2, 96, pages=8, page_size=16, graph=False)
+    assert model.embed.shape[0] == 1024
+    for call in (lambda: b.admit([[5, bad, 7]]), lambda: b.generate([[5], [bad]], 3)):
+        with pytest.raises(ValueError):
+            call()
+        assert whole(b, 8)
+    b.admit([[5, 0, 1023]])
+    free = len(b.pool.free)
+    with pytest.raises(ValueError):
+        b.verify({0: [3, bad]})
+    assert b.len[0] == 3 and len(b.pool.free) == free and len(b.verify({0: [0, 1023]})[0]) >= 1

@@ -126,6 +126,13 @@ class PagedBatch:
         return self._rows(flat, self._table[slots], i32(at), i32(cu), max(map(len, ids)),
                           max(a + len(t) for a, t in zip(at, ids)))
 
+    def _check_tokens(self, rows) -> None:
+        """The embedding is read on the device, where a token id past its end would fault."""
+        vocab = self.model.embed.shape[0]
+        for r in rows:
+            if r and not (0 <= min(r) and max(r) < vocab):
+                raise ValueError(f"token ids {min(r)} .. {max(r)}: the model has 0 .. {vocab - 1}")
+
     def _hold(self, slots: list[int], tokens: list[int]) -> None:
         if sum(self.pool.missing(s, t) for s, t in zip(slots, tokens)) > len(self.pool.free):
             raise UWCError(f"not enough pages: {len(self.pool.free)} free; release a sequence first")
@@ -147,6 +154,7 @@ class PagedBatch:
             raise ValueError(f"a prompt is empty or, with {reserve} tokens to come, longer than {self.max_len}")
         if chunk < 1 or reserve < 0:
             raise ValueError(f"chunk {chunk}, reserve {reserve}")
+        self._check_tokens(prompts)
         if not prompts:
             return {}
         self._hold(idle, [len(p) + reserve for p in prompts])
@@ -204,6 +212,7 @@ class PagedBatch:
             raise ValueError(f"slots {slots}: not all active")
         if any(self.len[s] + 1 + len(drafts[s]) > self.max_len for s in slots):
             raise ValueError(f"a slot's drafts end past max_len {self.max_len}")
+        self._check_tokens(drafts.values())
         self._hold(slots, [self.len[s] + 1 + len(drafts[s]) for s in slots])
         newest = self._tok.tolist()
         ids = [[newest[s]] + list(drafts[s]) for s in slots]
@@ -253,6 +262,7 @@ class PagedBatch:
                 raise ValueError(f"prompt {i} is empty or, with {more} tokens to cache, longer than {self.max_len}")
             if need[i] > len(self.pool.free):
                 raise UWCError(f"prompt {i} needs {need[i]} pages, of {len(self.pool.free)}")
+        self._check_tokens(prompts)
         out: list[list[int]] = [[] for _ in prompts]
         waiting, owner = list(range(len(prompts))), {}
         try:
