@@ -394,8 +394,9 @@ class MinedWeight:
         """(row_offset, col_offset, hash) of the winning tiles of the last call with this m (syncs).
         Raises if a kernel reported a device-side timeout since the last check."""
         words_ = self._wins_for(m).cpu().numpy().view(np.uint32)
-        st = _lib.device_status(clear=True)
-        if st:
+        st = _lib.device_status(clear=False)
+        if st & _lib.DEV_TIMEOUT:                     # other bits are their callers' to read (paged's DEV_RANGE)
+            _lib.device_status(clear=True)
             raise _lib.UWCError(f"device status {st:#x}: a kernel wait timed out; results are invalid")
         cnt = min(int(words_[0]), self.max_wins)
         return [(int(rec[0]), int(rec[1]), rec[2:].astype("<u4").tobytes())
