@@ -437,7 +437,8 @@ int uwc_stage_roots(const float* rows, int B, int T, int D, uint32_t* scratch, u
 /* ---- the paged 8-bit KV cache ------------------------------------------------------------------
  * New (the reference keeps one contiguous cache per batch, runtime/detrt/qwen3.py:216-221). One
  * layer's cache is a pool of pages: k, v (pages, Hkv, page_size, 128) int8, 16-byte aligned, and sk,
- * sv (pages, Hkv) float32, the scale of each (page, KV head); page_size 16, 32, 64 or 128. A cached
+ * sv (pages, Hkv) float32, the scale of each (page, KV head), finite and not negative (append writes no
+ * others); page_size 16, 32, 64 or 128. A cached
  * value is its integer times its page's scale.
  * A batch is ragged and described on the device, so one CUDA graph serves every step: rows cu[s] ..
  * cu[s + 1] - 1 of the row tensors are sequence s's new tokens (none where the two are equal) at
@@ -462,7 +463,8 @@ int uwc_stage_roots(const float* rows, int B, int T, int D, uint32_t* scratch, u
  * (128 float32 or NULL): det_rmsnorm of each head with eps before the rotation (Qwen3).
  * A page's scale is max(the scale of the tokens it already holds, max|new values| / 127); the tokens it
  * already holds are brought to a grown scale (rint(q * old / new)). Positions before start[s] in the
- * page of start[s] count as held; a page entered at its first position starts anew. Each step is one
+ * page of start[s] count as held; a page entered at its first position starts anew. A call sets its
+ * sequences' ends: tokens that a page held past start[s] + new ones are given up. Each step is one
  * IEEE float32 operation. Infinities are stored as +-127 and NaN as 0; neither counts toward the scale. */
 int uwc_paged_append(int8_t* kc, float* sk, int8_t* vc, float* sv, int pages, int page_size, int Hkv,
                      const int* table, const int* start, const int* cu, int seqs, int width, int rows, int max_new,

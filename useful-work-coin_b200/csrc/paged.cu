@@ -7,7 +7,8 @@
 //                    and an old token's q becomes rint(fdiv(fmul(q, s0), s)) when s > s0. Every step
 //                    is one IEEE operation, the rotation too (fadd(fmul(x, cos), fmul(rot(x), sin))),
 //                    so a cache is the same bit for bit wherever and in whatever batch it was written,
-//                    and appending the same tokens again changes nothing.
+//                    and appending a sequence's newest tokens again changes nothing. A call sets the sequence's
+//                    end: tokens that its last page held past it are not brought to a scale that grows or starts anew.
 //   k_paged_gather   cached tokens back as 16- or 32-bit values.
 //
 // Both are bound by HBM at prompt sizes and by latency at decode sizes. Measured on B200 (a graph of calls): 8
@@ -162,7 +163,7 @@ __device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv, f
 }
 __device__ __forceinline__ float inverse(float s) { return s > 1e-30f ? __frcp_rn(s) : __int_as_float(0x7f800000); }
 
-// One row of queries: unit u is (row, four query heads) of eight lanes, four units a warp.
+// One row of queries: unit u is (row, kQHeads query heads) of eight lanes, four units a warp.
 template <typename T, bool NORM>
 __device__ __forceinline__ void query_unit(const AppendArgs& a, long long u, int c) {
   const int groups = (a.H + kQHeads - 1) / kQHeads;
@@ -215,7 +216,7 @@ __device__ __forceinline__ void query_unit(const AppendArgs& a, long long u, int
     }
     return;
   }
-  // in place, four dims of all four heads at a time: the rotation values are read once
+  // in place, four dims of all its heads at a time: the rotation values are read once
   if (pos >= 0) {
 #pragma unroll
     for (int k = 0; k < 2; k++) {
@@ -330,9 +331,13 @@ __device__ __forceinline__ void unpack4(const Raw& r, int k, float* lo, float* h
 
 // Prompts: one CTA a page unit of HP heads, its rows in NP passes of TH / 8. All rows' loads are issued first
 // and stay packed (16 bits); without a norm a key is rotated twice, for the maximum and for its quantization,
-// which costs less than the registers that would hold it: at 64 registers instead of 86 the SM has four CTAs'
-// loads in flight, not two. Two heads share the rotation values, which are four times a key's bytes (13 x up
-// to 777 tokens of 12 + 2 x 4 heads, pages of 16: 13.2 us instead of 15.2). Pages of 16 have CTAs of half the size: half of 256 threads had no row.
+// which costs less than the registers that would hold it (80 for pages of 64 and 128, three CTAs an SM; 64 for
+// pages of 16 and 32, four). What bounds it is latency at that occupancy: a CTA loads, waits for its maximum,
+// stores and leaves, nothing of which overlaps inside it. Of 8 prompts of 2048's 63 us the schedulers issue in 55 %
+// of the cycles, with a third of the warps resident and DRAM at 38 %. Two heads share the rotation values, which are
+// four times a key's bytes (13 x up to 777 tokens of 12 + 2 x 4 heads, pages of 16: 13.2 us instead of 15.2). Pages
+// of 16 have CTAs of half the size: half of 256 threads had no row. A norm takes a head's 128 values at once and runs
+// in both passes: 135 us with norms where it is 62 without.
 template <typename T, int NP, int TH, int HP, bool NORM>
 __global__ void __launch_bounds__(TH, (NORM ? 2 : NP * HP == 4 ? 3 : 4) * kThreads / TH) k_paged_append(const AppendArgs a) {
   const int tid = threadIdx.x, c = tid & 7, r8 = tid >> 3;
@@ -439,7 +444,9 @@ __global__ void __launch_bounds__(TH, (NORM ? 2 : NP * HP == 4 ? 3 : 4) * kThrea
 }
 
 // Decode steps (at most kFewNew new tokens a sequence): one warp a page unit, so that a batch's units are
-// all resident at once and none waits at a barrier.
+// all resident at once and none waits at a barrier. Eight is what two rows a lane hold; against the page kernel (32 + 2 x 8
+// heads): 64 sequences with 1 new token 4.6 us and 8.7 (pages of 64; of 16: 4.2 and 5.3), with 4 4.9 and 8.8, with 8
+// 6.7 and 9.7 (6.2 either way); with norms 5.7 and 17 for 1 token.
 constexpr int kFewNew = 8;
 constexpr int kFewThreads = 128;
 template <typename T, bool NORM>

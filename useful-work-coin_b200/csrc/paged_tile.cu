@@ -377,7 +377,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_tile(const TileArgs ta) {
     const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + 256 + w * 128;
     const float inv_g = 1.0f / (float)G;
     uint32_t it = 0, all = 0, wgp = 0;             // this warpgroup's tiles, every tile, its barrier's phases
-#pragma unroll 1
     // Row x of an item is token (x + rem) / G past the item's first one: a division of small numbers, exact in
     // float32 while they are below 2^20.
     auto token_of = [&](int x) { return (int)(((float)x + 0.5f) * inv_g); };

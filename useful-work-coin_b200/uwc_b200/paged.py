@@ -50,7 +50,10 @@ def append(k, v, cache: dict, table, start, cu, max_new: int, cos, sin, q=None, 
     the rotation (Qwen3). max_new: a bound on a sequence's new tokens.
 
     A page's scale is its largest magnitude / 127: it grows when a new token needs it, and the tokens
-    already there are brought to it. Appending the same tokens again changes nothing."""
+    already there, at positions before start[s], are brought to it. Appending a sequence's newest tokens
+    again changes nothing. start[s] + new tokens is then the sequence's end: what a page held past it (drafts
+    that were rejected, a longer sequence rolled back) is given up and no longer stands for its values, so an
+    earlier chunk is not written again under tokens that are to stay."""
     return _paged.append(cache["k"], cache["v"], cache["sk"], cache["sv"], table, start, cu, max_new, k, v, cos, sin, q,
                          q_norm, k_norm, eps)
 

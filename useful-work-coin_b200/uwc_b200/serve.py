@@ -58,8 +58,9 @@ class PagePool:
 
 class PagedBatch:
     """`slots` sequences of up to max_len tokens on one DetQwen3's weights. pages: pages of a layer's pool (by
-    default enough for every slot at max_len). window / sinks: as in paged.attention. graph: a step is replayed
-    as one CUDA graph. The caller serializes its calls, as for DecodeGraph."""
+    default enough for every slot at max_len). window / sinks: as in paged.attention (DetQwen3 takes no checkpoint
+    trained with a window below max_pos, so that a window here approximates a model of full attention; its hidden
+    pages stay held). graph: a step is replayed as one CUDA graph. The caller serializes its calls, as for DecodeGraph."""
 
     def __init__(self, model, slots: int, max_len: int, pages: int | None = None, page_size: int = 64,
                  window: int | None = None, sinks: int = 0, graph: bool = True):
@@ -182,7 +183,7 @@ class PagedBatch:
 
     @torch.no_grad()
     def step(self) -> dict[int, int]:
-        """The next greedy token of every active slot."""
+        """The next greedy token of every active slot; refused while one of them holds max_len tokens."""
         act = self.active()
         if not act:
             return {}
