@@ -106,3 +106,21 @@ def test_tokens_that_the_model_has_not_are_refused(dev, model, bad):
     with pytest.raises(ValueError):
         b.verify({0: [3, bad]})
     assert b.len[0] == 3 and len(b.pool.free) == free and len(b.verify({0: [0, 1023]})[0]) >= 1
+
+
+def test_prompts_and_drafts_of_any_sequence_type(dev, model):
+    """Lists, tuples, arrays and tensors of token ids."""
+    import numpy as np
+    from uwc_b200.serve import PagedBatch
+    ps = prompts(20, 3)
+    b = PagedBatch(model, 2, 96, pages=8, page_size=16, graph=False)
+    want = b.generate(ps, 4)
+    for make in (tuple, np.array, torch.tensor):
+        assert b.generate([make(p) for p in ps], 4) == want
+        b.admit([make(p) for p in ps])
+        said = b.verify({0: make(want[0][1:3]), 1: make([])})
+        assert said[0] == want[0][1:4] and said[1] == want[1][1:2]
+        b.release(0)
+        b.release(1)
+        with pytest.raises(ValueError):
+            b.admit([make([7, 1024])])

@@ -131,7 +131,7 @@ class PagedBatch:
         """The embedding is read on the device, where a token id past its end would fault."""
         vocab = self.model.embed.shape[0]
         for r in rows:
-            if r and not (0 <= min(r) and max(r) < vocab):
+            if len(r) and not (0 <= min(r) and max(r) < vocab):
                 raise ValueError(f"token ids {min(r)} .. {max(r)}: the model has 0 .. {vocab - 1}")
 
     def _hold(self, slots: list[int], tokens: list[int]) -> None:
@@ -259,7 +259,7 @@ class PagedBatch:
         more = n_new - 1                              # the last token is answered, not cached
         need = [-(-(len(p) + more) // self.pool.page_size) for p in prompts]
         for i, p in enumerate(prompts):
-            if not p or len(p) + more > self.max_len:
+            if len(p) == 0 or len(p) + more > self.max_len:
                 raise ValueError(f"prompt {i} is empty or, with {more} tokens to cache, longer than {self.max_len}")
             if need[i] > len(self.pool.free):
                 raise UWCError(f"prompt {i} needs {need[i]} pages, of {len(self.pool.free)}")
